@@ -151,7 +151,7 @@ def prepare(case, seed):
                         torch.randn(places, case["item"], generator=g, device=DEV, dtype=dtype))
         order = torch.randperm(places, generator=host)
         return {"case": case, "pools": [make() for _ in range(case["pools"])],
-                "sources": order[:case["pairs"]].int().to(DEV), "targets": order[case["pairs"]:2 * case["pairs"]].int().to(DEV)}
+                "sources": order[:case["pairs"]].tolist(), "targets": order[case["pairs"]:2 * case["pairs"]].tolist()}
     dtype, hq, hk, block = getattr(torch, case["dtype"]), case["heads"], case["kv_heads"], case["block"]
     if case["kind"] == "decode":
         ends = _contexts(case)
@@ -266,7 +266,7 @@ def _attend(q, k, v, mask):
 def _plain(s):
     case = s["case"]
     if case["kind"] == "pages":
-        a, b = s["sources"].long(), s["targets"].long()
+        a, b = torch.tensor([s["sources"], s["targets"]]).to(DEV)
         return [p.index_copy_(0, b, p[a]) for p in s["pools"]]
     dtype, hq, hk, block = getattr(torch, case["dtype"]), case["heads"], case["kv_heads"], case["block"]
     R = hq // hk
@@ -349,7 +349,7 @@ def exact(case, seed):
         out = []
         for p in s["pools"]:
             p = p.double()
-            for a, b in zip(s["sources"].tolist(), s["targets"].tolist()):
+            for a, b in zip(s["sources"], s["targets"]):
                 p[b] = p[a]
             out.append(p)
         return out
