@@ -37,7 +37,8 @@ enum {
   NQB200_ERR_UNSUPPORTED_DEVICE = 6, /* not compute capability 10.x */
   NQB200_ERR_LAUNCH = 7,        /* the CUDA runtime refused the launch */
   NQB200_ERR_WAIT_TIMEOUT = 8,  /* a bounded device-side wait gave up */
-  NQB200_ERR_TOO_LARGE = 9      /* a size exceeds a stated maximum */
+  NQB200_ERR_TOO_LARGE = 9,     /* a size exceeds a stated maximum */
+  NQB200_ERR_BAD_INDEX = 10     /* a page, cache row or position lies outside its buffer */
 };
 
 enum { NQB200_F16 = 0, NQB200_BF16 = 1 };
@@ -207,6 +208,64 @@ int nqb200_decode_attention_split(const void* qkv, int64_t row_stride, const voi
                                   const int32_t* ctx, int64_t table_width, int64_t block_size, void* out, int64_t batch, int64_t num_q_heads,
                                   int64_t num_kv_heads, int64_t head_dim, float scale, float eps, int dtype, void* scratch, size_t scratch_bytes,
                                   void* stream);
+
+/* ---- key/value cache of 4 bits, heads of 128 ----------------------------------------------------------------
+ * A page holds block_size rows (a multiple of 16) of every key/value head: k and v are [pages, kv_heads, block_size * 72] bytes.  The
+ * 72 * block_size bytes of a page and head are block_size rows of 64 bytes, then block_size rows of four numbers of the model's
+ * 16-bit type: scale and offset of dimensions 0..63, scale and offset of dimensions 64..127.  The 32-bit word 2 m + j of a row holds
+ * dimensions 64 j + 8 m .. + 7: dimension 2 i of the eight is nibble i, dimension 2 i + 1 nibble i + 4.  A nibble n stands for
+ * offset + n * scale.  Quantising takes the group's smallest value as offset and a fifteenth of its range as scale, both rounded to
+ * the 16-bit type, and the nearest n; a group with a value that is not finite, or whose range is beyond float, reads back as NaN.
+ * Cache row r is row r % block_size of page r / block_size.
+ *
+ * No kernel follows an index out of its buffer.  A page, row or position that lies outside is reported in *status (an int on the
+ * device that takes NQB200_ERR_BAD_INDEX; may be NULL): such a row is not stored and reads back as zeros, such a page's keys are left
+ * out, such a position is taken as 0.  No counterpart in the reference (it has no cache). */
+typedef struct nqb200_kv4 {
+  void* k;
+  void* v;
+  int64_t pages;
+  int64_t kv_heads;
+  int64_t block_size;
+} nqb200_kv4;
+
+/* Tokens of a prompt step: q_out [T, num_q_heads * 128] takes the queries of qkv [T, row_stride] after head norm and rotation (as
+ * nqb200_qknorm_rope, but computed in 32 bits and rounded once), cache row rows[t] takes the keys, normed and rotated, and the values.
+ * A row below 0: the token is not stored.  qkv is left as it is.  cos_sin: [max_positions, 128].  row_stride a multiple of 4. */
+int nqb200_kv4_store(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+                     int64_t max_positions, const int64_t* positions, const int64_t* rows, const nqb200_kv4* cache, void* q_out, int64_t T,
+                     int64_t num_q_heads, float eps, int dtype, int* status, void* stream);
+/* The values of cache rows, rounded to the 16-bit type: k_out and v_out [n, kv_heads, 128].  A row below 0 gives zeros. */
+int nqb200_kv4_load(const nqb200_kv4* cache, const int64_t* rows, void* k_out, void* v_out, int64_t n, int dtype, int* status, void* stream);
+
+/* nqb200_decode_attention over such a cache: norm, rotation and store of one token per sequence, then attention over ctx[b] keys, the
+ * token's own among them (as it is stored).  table [batch, table_width].  ctx[b] = 0 is a row without a sequence: zeros, and nothing of
+ * its table, row and position is read.  rows[b] < 0: the token is attended to and not stored. */
+int nqb200_kv4_decode_attention(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
+                                int64_t max_positions, const int64_t* positions, const int64_t* rows, const nqb200_kv4* cache,
+                                const int32_t* table, int64_t table_width, const int32_t* ctx, void* out, int64_t batch,
+                                int64_t num_q_heads, float scale, float eps, int dtype, void* scratch, size_t scratch_bytes, int* status,
+                                void* stream);
+/* Bytes of scratch of that call: written before read, not shared by calls that can overlap. */
+size_t nqb200_kv4_decode_scratch_bytes(int64_t table_width, int64_t block_size, int64_t batch, int64_t num_q_heads, int64_t kv_heads);
+
+/* Causal attention of several tokens per sequence over the cache, which holds their own keys and values too: tokens cu[b] ..
+ * cu[b + 1] - 1 of q [T, q_stride] stand at positions pos0[b] .. of sequence b, and each sees all positions up to its own.  out [T,
+ * num_q_heads * 128].  What the host knows of the lengths (a bound each; cu and pos0 say the rest): max_len tokens of a sequence, max_ctx keys
+ * of one, and the sum over the sequences of their keys' tiles of 128 (`tiles`).  A sequence beyond them is reported as a bad index.
+ * q_stride a multiple of 8. */
+int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, const nqb200_kv4* cache, const int32_t* table, int64_t table_width,
+                                const int32_t* cu, const int32_t* pos0, void* out, int64_t batch, int64_t T, int64_t max_len,
+                                int64_t max_ctx, int64_t tiles, int64_t num_q_heads, float scale, int dtype, void* scratch,
+                                size_t scratch_bytes, int* status, void* stream);
+size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads,
+                                       int64_t kv_heads);
+
+/* Copies of pages, or of any rows of equal size: for every pool p and pair i, row_bytes[p] bytes from row sources[i] to row
+ * targets[i] of pools[p], all on one device.  The numbers are read during the call (host memory).  The same target twice, or a
+ * target that is also a source, is refused, as is a row outside [0, rows). */
+int nqb200_copy_pages(void* const* pools, const int64_t* row_bytes, int64_t n_pools, int64_t rows, const int32_t* sources,
+                      const int32_t* targets, int64_t n_pairs, void* stream);
 
 /* One-shot all-reduce (sum) over NVLink peer memory for the small [M, N] partial results of a
  * row-parallel linear.  No counterpart in the reference (it has no distributed code).

@@ -26,6 +26,12 @@ class DecodeFusion(ctypes.Structure):
                 ("ssq_out", ctypes.c_void_p)]
 
 
+class Kv4(ctypes.Structure):
+    """nqb200_kv4 of include/nqb200.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("block_size", ctypes.c_int64)]
+
+
+_kv4 = ctypes.POINTER(Kv4)
 FUSE_RMSNORM, FUSE_RESIDUAL, FUSE_SILU_MUL, FUSE_ALLREDUCE = 1, 2, 4, 8
 
 # name -> (restype, argtypes); mirrors include/nqb200.h one to one
@@ -52,6 +58,14 @@ SIGNATURES = {
     "nqb200_decode_attention": (_int, [_vp, _i64] + [_vp] * 9 + [_i64, _i64, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_float, _int, _vp]),
     "nqb200_decode_attention_scratch_bytes": (_sz, [_i64] * 5),
     "nqb200_decode_attention_split": (_int, [_vp, _i64] + [_vp] * 9 + [_i64, _i64, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_float, _int, _vp, _sz, _vp]),
+    "nqb200_kv4_store": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _kv4, _vp, _i64, _i64, ctypes.c_float, _int, _vp, _vp]),
+    "nqb200_kv4_load": (_int, [_kv4, _vp, _vp, _vp, _i64, _int, _vp, _vp]),
+    "nqb200_kv4_decode_attention": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _kv4, _vp, _i64, _vp, _vp, _i64, _i64, ctypes.c_float, ctypes.c_float, _int,
+                                           _vp, _sz, _vp, _vp]),
+    "nqb200_kv4_decode_scratch_bytes": (_sz, [_i64] * 5),
+    "nqb200_kv4_prompt_attention": (_int, [_vp, _i64, _kv4, _vp, _i64, _vp, _vp, _vp] + [_i64] * 6 + [ctypes.c_float, _int, _vp, _sz, _vp, _vp]),
+    "nqb200_kv4_prompt_scratch_bytes": (_sz, [_i64] * 7),
+    "nqb200_copy_pages": (_int, [ctypes.POINTER(_vp), ctypes.POINTER(_i64), _i64, _i64, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), _i64, _vp]),
     "nqb200_silu_mul": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "nqb200_comm_alloc": (_int, [ctypes.POINTER(_vp), _sz]),
     "nqb200_comm_free": (_int, [_vp]),
@@ -207,7 +221,7 @@ def load_moe() -> ctypes.CDLL:
 
 
 _STATUS = ("ok", "bad shape", "bad dtype", "misaligned pointer", "null pointer", "workspace missing or too small",
-           "unsupported device", "CUDA launch failed", "a bounded device-side wait timed out", "size exceeds the supported maximum")
+           "unsupported device", "CUDA launch failed", "a bounded device-side wait timed out", "size exceeds the supported maximum", "a page, cache row or position lies outside its buffer")
 
 
 def check_mixers(status: int) -> None:
@@ -233,6 +247,49 @@ def check_mixer_status() -> None:
         if status != 0:
             word.zero_()
             check_mixers(status)
+
+
+class on_device:
+    """Makes a tensor's device the current one for a call; gives the device's index and its current stream."""
+    __slots__ = ("index", "before", "stream")
+
+    def __init__(self, dev: torch.device):
+        self.before = torch.cuda.current_device()
+        self.index = self.before if dev.index is None else dev.index
+
+    def __enter__(self):
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        self.stream = stream_of(self.index)
+        return self
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+_cache_status: dict[int, torch.Tensor] = {}
+
+
+def cache_status(device: int) -> int | None:
+    """Address of the device's status word of the 4-bit cache's kernels (0: no bad index, no wait that gave up).  None in a
+    stream capture that comes before the device's first call, since the word cannot be made there."""
+    word = _cache_status.get(device)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        word = _cache_status[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+        torch.cuda.current_stream(device).synchronize()      # other streams' kernels may be the next to use it
+    return word.data_ptr()
+
+
+def check_cache_status() -> None:
+    """Synchronise and raise if a kernel of the 4-bit cache met a page, row or position outside its buffer; the word is cleared."""
+    for word in _cache_status.values():
+        status = int(word.item())
+        if status != 0:
+            word.zero_()
+            check(status)
 
 
 def mixer_dtype_code(dtype: torch.dtype) -> int:

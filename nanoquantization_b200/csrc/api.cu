@@ -21,6 +21,7 @@ extern "C" const char* nqb200_status_string(int status) {
     case NQB200_ERR_LAUNCH: return "CUDA launch failed";
     case NQB200_ERR_WAIT_TIMEOUT: return "a bounded device-side wait timed out";
     case NQB200_ERR_TOO_LARGE: return "size exceeds the supported maximum";
+    case NQB200_ERR_BAD_INDEX: return "a page, cache row or position lies outside its buffer";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,103 @@
+"""The 4-bit cache and copies of pages without a GPU: refusals at the C entries and in Python, and the layout's own reference."""
+import ctypes
+
+import pytest
+import torch
+
+from nanoquantization_b200 import _lib
+from nanoquantization_b200.layers import kv4, pages
+from tests import kv4_reference as ref
+
+
+def _c(pages_=4, heads=2, block=16, k=1 << 20, v=1 << 20):
+    return _lib.Kv4(k, v, pages_, heads, block)
+
+
+P = 1 << 20        # an address that is aligned and never reached
+
+
+def test_refusals_of_the_store_and_the_read_back():
+    lib = _lib.load()
+
+    def store(cache=None, qkv=P, stride=8 * 128, qw=P, cs=P, maxpos=10, rows=P, out=P, T=1, heads=4, dtype=0):
+        return lib.nqb200_kv4_store(qkv, stride, qw, P, cs, maxpos, P, rows, cache or _c(), out, T, heads, 1e-6, dtype, None, None)
+    assert lib.nqb200_kv4_store(P, 1024, P, P, P, 10, P, P, None, P, 1, 4, 1e-6, 0, None, None) == 4
+    for bad in (_c(0), _c(-1), _c(1 << 31), _c(heads=0), _c(heads=4097), _c(block=0), _c(block=24), _c(block=-16)):
+        assert store(bad) == 1
+        assert lib.nqb200_kv4_load(bad, P, P, P, 1, 0, None, None) == 1
+    assert store(_c(k=None)) == store(_c(v=0)) == 4 and store(_c(k=P + 8)) == 3
+    assert store(T=-1) == store(heads=0) == store(maxpos=0) == store(stride=8 * 128 - 4) == store(stride=8 * 128 + 2) == 1
+    assert store(dtype=2) == store(dtype=-1) == 2
+    assert store(T=0, qkv=None) == 0 and store(T=1 << 31) == 9
+    assert store(qkv=None) == store(qw=None) == store(cs=None) == store(rows=None) == store(out=None) == 4
+    assert store(qkv=P + 4) == store(qw=P + 2) == store(cs=P + 8) == store(out=P + 4) == 3
+
+    def load(n=1, rows=P, k=P, v=P, dtype=0):
+        return lib.nqb200_kv4_load(_c(), rows, k, v, n, dtype, None, None)
+    assert load(-1) == 1 and load(dtype=2) == 2 and load(0, None) == 0 and load(1 << 31) == 9
+    assert load(rows=None) == load(k=None) == load(v=None) == 4 and load(k=P + 8) == load(v=P + 8) == 3
+
+
+def test_refusals_of_the_attention():
+    lib = _lib.load()
+
+    def decode(cache=None, qkv=P, stride=8 * 128, maxpos=10, rows=P, table=P, width=3, ctx=P, out=P, batch=1, heads=4, dtype=0, scratch=P, nbytes=1 << 40):
+        return lib.nqb200_kv4_decode_attention(qkv, stride, P, P, P, maxpos, P, rows, cache or _c(), table, width, ctx, out, batch, heads, 0.1, 1e-6, dtype, scratch, nbytes, None, None)
+    assert decode(_c(block=8)) == decode(heads=3) == decode(heads=0) == decode(width=0) == decode(width=1 << 31) == decode(batch=-1) == decode(batch=65536) == 1
+    assert decode(stride=7 * 128) == decode(stride=8 * 128 + 4) == decode(maxpos=0) == 1
+    assert decode(dtype=2) == 2 and decode(batch=0, qkv=None) == 0
+    assert decode(qkv=None) == decode(rows=None) == decode(table=None) == decode(ctx=None) == decode(out=None) == 4
+    assert decode(qkv=P + 8) == decode(out=P + 8) == 3
+
+    def prompt(cache=None, q=P, stride=512, table=P, width=3, cu=P, out=P, batch=1, T=4, max_len=4, max_ctx=4, tiles=1, heads=4, dtype=0, scratch=P, nbytes=1 << 40):
+        return lib.nqb200_kv4_prompt_attention(q, stride, cache or _c(), table, width, cu, P, out, batch, T, max_len, max_ctx, tiles, heads, 0.1, dtype, scratch, nbytes, None, None)
+    assert prompt(_c(block=8)) == prompt(heads=3) == prompt(width=0) == prompt(batch=-1) == prompt(batch=65536) == prompt(T=-1) == prompt(max_len=-1) == 1
+    assert prompt(max_ctx=3) == prompt(tiles=-1) == prompt(stride=504) == prompt(stride=516) == 1
+    assert prompt(dtype=7) == 2 and prompt(batch=0, q=None) == prompt(T=0, q=None) == 0
+    assert prompt(q=None) == prompt(table=None) == prompt(cu=None) == prompt(out=None) == 4 and prompt(q=P + 8) == prompt(out=P + 8) == 3
+
+
+def test_refusals_of_the_copies():
+    lib = _lib.load()
+
+    def copy(src, dst, rows=8, pools=(P,), nbytes=(16,)):
+        n, m = len(src), len(pools)
+        return lib.nqb200_copy_pages((ctypes.c_void_p * m)(*pools), (ctypes.c_int64 * m)(*nbytes), m, rows, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, None)
+    assert copy([], []) == 0 and copy([0], [1], pools=(), nbytes=()) == 0
+    assert copy([0], [1], rows=0) == copy([0], [1], nbytes=(0,)) == 1 and copy([0], [1], pools=(None,)) == 4
+    # out of range, a target twice, a target that is a source
+    for src, dst in (([-1], [1]), ([8], [1]), ([0], [-1]), ([0], [8]), ([0, 2], [1, 1]), ([0, 1], [1, 2]), ([3], [3]), ([0] * 9, list(range(9)))):
+        assert copy(src, dst) == 10
+    assert lib.nqb200_copy_pages(None, None, 1, 8, None, None, 1, None) == 4
+
+
+def test_refusals_in_python():
+    with pytest.raises(ValueError, match="multiple of 16"):
+        kv4.new_cache(2, 24, 1, "cpu")
+    kc, vc = kv4.new_cache(2, 32, 3, "cpu")
+    assert kc.shape == vc.shape == (2, 3, 32 * 72) and kc.dtype == torch.uint8 and not kc.any()
+    x = torch.zeros(1, 9 * 128, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        kv4.load(kc, vc, torch.zeros(1, dtype=torch.int64), torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        kv4.prompt_attention(x, 9, kc, vc, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), [1], [0])
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        pages.copy_pages([kc], [0], [1])
+    with pytest.raises(ValueError, match="1 sources and 2 targets"):
+        pages.copy_pages([kc], [0], [1, 2])
+    pages.copy_pages([], [], [])
+    pages.copy_pages([kc], [], [])
+    for bad in ((kc.float(), vc), (kc, vc[:, :2]), (kc[:, :, :-72], vc[:, :, :-72]), (kc.transpose(0, 1), vc.transpose(0, 1)), (kc[0], vc[0])):
+        with pytest.raises((TypeError, ValueError), match="4-bit cache"):
+            kv4._cache(*bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_layout_reads_back_what_it_packs(dtype):
+    x = torch.randn(40, 128, generator=torch.Generator().manual_seed(0), dtype=torch.float64)
+    assert torch.equal(ref.unpack(*ref.pack(x, dtype), dtype), ref.quantised(x, dtype))
+    assert float((ref.quantised(x, dtype) - x).abs().max()) <= float(ref.params_of(x, dtype)[0].max()) * 0.6
+
+
+def test_a_zero_filled_cache_reads_as_zeros():
+    assert not ref.unpack(torch.zeros(3, 64, dtype=torch.uint8), torch.zeros(3, 8, dtype=torch.uint8), torch.float16).any()
