@@ -219,8 +219,8 @@ int nqb200_decode_attention_split(const void* qkv, int64_t row_stride, const voi
  * Cache row r is row r % block_size of page r / block_size.
  *
  * No kernel follows an index out of its buffer.  A page, row or position that lies outside is reported in *status (an int on the
- * device that takes NQB200_ERR_BAD_INDEX; may be NULL): such a row is not stored and reads back as zeros, such a page's keys are left
- * out, such a position is taken as 0.  No counterpart in the reference (it has no cache). */
+ * device that takes NQB200_ERR_BAD_INDEX; may be NULL): such a row is not stored, it and the rows of such a page read as zeros, and
+ * such a position is taken as 0.  No counterpart in the reference (it has no cache). */
 typedef struct nqb200_kv4 {
   void* k;
   void* v;

@@ -1,14 +1,39 @@
-// Attention over the 4-bit key/value cache: one token per sequence (with norm, rotation and store of that token), and several.
+// Attention over the 4-bit key/value cache for few queries: one token per sequence, with its norm, rotation and store in the same
+// launch, and a few tokens per sequence (drafts, ends of prompts).
 //
-// A CTA takes a query head of a token; its warps take keys in turn, a lane four dimensions of each, and keep a running maximum and sum.
+// Bound by reading the visible keys and values once (144 bytes per key and head) and, next to it, by the instructions that take
+// nibbles apart.  A CTA takes up to eight columns of a key/value head (query heads of a token, or of several tokens) and a share of the keys; its warps
+// take tiles of 32 keys on their own, through rings that they fill with cp.async.  Both products are mma m16n8k16 with the columns as the
+// eight columns of its result:
+//
+//   numbers  a nibble n becomes 1 + n/16, one shift and one logical operation for a pair: the nibble goes into the mantissa of 1.
+//            Nothing is subtracted and nothing scaled before a product.  With S = 16 scale and T = offset - S a value is S (1 + n/16) + T.
+//   scores   per group of 64 dimensions the product c of the lifted key and the query, then score = S0 c0 + S1 c1 + T0 q0 + T1 q1,
+//            q0 and q1 the sums of the query's halves, all in float.  Keys are exact; the query is the only thing that is rounded.
+//   values   the weight times the value's scale goes into the product, rounded once, a version for each of the two groups; the product
+//            with a matrix of ones gives the sum of just these rounded weights, and 16 (product - sum) + sum(weight offset) is the result.
+//            With float16 the scales are taken relative to the largest that the warp has seen, so that tiny values keep their bits.
+//   order    a lane owns 16 neighbouring bytes of a key and 8 of a value, which one load fetches; which dimension is which row of a
+//            product follows from that, as the layout of a row was chosen.
+//
+// The running maximum of a column moves only when a score is 8 (in log2 units) above it, found by one vote per 32 keys.  The warps meet in
+// shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
+#include <cooperative_groups.h>
+#include <type_traits>
 #include "kv4.cuh"
 
 namespace nqb200 {
 namespace {
 
 using namespace kv4;
-constexpr int kWarps = 4;
-constexpr float kLog2e = 1.4426950408889634f;
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32, kCols = 8;
+constexpr int kStage = kTile * 2 * kToken;                    // keys, values, parameters of keys, parameters of values
+constexpr int kOffV = kTile * kData, kOffKP = 2 * kTile * kData, kOffVP = kOffKP + kTile * kParams;
+constexpr int kOS = kDim + 4;                                 // floats of a column's partial sums
+constexpr int kShare = kDim + 4;                              // floats of a column's share: sums, maximum, sum of weights
+constexpr float kLog2e = 1.4426950408889634f, kLag = 8.f;
 
 struct Args {
   const uint16_t* q; int64_t stride;              // queries, or the projections of a decode step
@@ -16,138 +41,553 @@ struct Args {
   const float* cos_sin; int64_t max_positions;
   const int64_t *positions, *rows;
   Cache cache;
-  const int32_t* table; int64_t width;
-  const int32_t *ctx, *cu, *pos0;
+  const int32_t* table; int width;
+  const int32_t *ctx;                             // decode
+  const int32_t *cu, *pos0;                       // several tokens per sequence
   uint16_t* out;
-  int batch, heads, max_len, max_ctx;
+  int heads, groups, tokens, max_len;             // groups: of kCols columns, per key/value head
   float scale, eps;
+  float* shares; int parts;                       // a sequence over several clusters (parts > 1): their shares
   int* status;
 };
 
-// Four dimensions 4 lane .. + 3 of a stored row.
-template <bool BF16> __device__ __forceinline__ void fetch(const uint32_t* row, uint2 params, float (&x)[4]) {
-  const int lane = threadIdx.x & 31, j = lane >> 4, m = (lane & 15) >> 1, half = lane & 1;
-  const uint32_t word = row[2 * m + j], p = j ? params.y : params.x;
-  const float s = scale_of<BF16>(p), off = offset_of<BF16>(p);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = fmaf(nibble(word, 2 * half + (e >> 1) + 4 * (e & 1)), s, off);
+struct Fixed {                                    // behind the rings
+  alignas(16) uint16_t q[kCols][kDim + 8];
+  alignas(16) uint32_t own[2][kData / 4];         // the step's own key and value, as stored
+  uint2 own_params[2];
+  float m[kWarps][kCols], l[kWarps][kCols];
+  float cm[kCols], cl[kCols];                     // of the CTA, read by the cluster
+  float out[kCols][kDim];
+};
+__host__ __device__ constexpr int ring_bytes(int stages) { return kWarps * stages * kStage; }
+constexpr int smem_bytes(int stages) { return ring_bytes(stages) + (int)sizeof(Fixed); }
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {      // zeros behind `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// Nibbles I and I + 4 of a word as 1 + n/16 in both halves.
+template <bool BF16, int I> __device__ __forceinline__ uint32_t lift(uint32_t w) {
+  constexpr int to = BF16 ? 3 - 4 * I : 6 - 4 * I;
+  const uint32_t x = to > 0 ? w << (to > 0 ? to : 0) : w >> (to > 0 ? 0 : -to);
+  return BF16 ? (x & 0x00780078u) | 0x3F803F80u : (x & 0x03C003C0u) | 0x3C003C00u;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF16) { const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&v); }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <bool BF16, bool DECODE>
-__global__ void __launch_bounds__(32 * kWarps) kv4_rows_kernel(const __grid_constant__ Args a) {
-  __shared__ __align__(16) uint32_t own[2][kData / 4];
-  __shared__ uint2 own_params[2];
-  __shared__ float s_q[kDim], s_o[kWarps][kDim], s_m[kWarps], s_l[kWarps];
+// A head after norm and rotation: half a warp, lane l has dimensions 4 l .. and 64 + 4 l ..; `weight` null: as it is.
+template <bool BF16>
+__device__ __forceinline__ void turned(const uint16_t* src, const uint16_t* weight, const float* angles, float eps, float (&x)[4], float (&y)[4]) {
+  const int l = threadIdx.x & 15;
+  const uint2 lo = reinterpret_cast<const uint2*>(src)[l], hi = reinterpret_cast<const uint2*>(src)[l + 16];
+  const uint32_t lw[2] = {lo.x, lo.y}, hw[2] = {hi.x, hi.y};
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = raw16_to_float<BF16>((uint16_t)(lw[e >> 1] >> (16 * (e & 1))));
+    y[e] = raw16_to_float<BF16>((uint16_t)(hw[e >> 1] >> (16 * (e & 1))));
+    ss += x[e] * x[e] + y[e] * y[e];
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+  if (!weight) return;
+  const float inv = rsqrtf(ss / (float)kDim + eps);
+  const uint2 wl = reinterpret_cast<const uint2*>(weight)[l], wh = reinterpret_cast<const uint2*>(weight)[l + 16];
+  const uint32_t wlw[2] = {wl.x, wl.y}, whw[2] = {wh.x, wh.y};
+  const float4 cv = reinterpret_cast<const float4*>(angles)[l], sv = reinterpret_cast<const float4*>(angles)[l + 16];
+  const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float u = x[e] * inv * raw16_to_float<BF16>((uint16_t)(wlw[e >> 1] >> (16 * (e & 1))));
+    const float v = y[e] * inv * raw16_to_float<BF16>((uint16_t)(whw[e >> 1] >> (16 * (e & 1))));
+    x[e] = u * c[e] - v * s[e];
+    y[e] = u * s[e] + v * c[e];
+  }
+}
+
+// STAGES: tiles of a warp's ring (see split()).  DECODE: one token per sequence whose own key and value are made here.
+template <bool BF16, bool DECODE, int STAGES>
+__global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel(const __grid_constant__ Args a) {
+  constexpr int kRing = ring_bytes(STAGES);
+  extern __shared__ __align__(128) uint8_t smem[];
+  Fixed& fx = *reinterpret_cast<Fixed*>(smem + kRing);
   grid_launch_dependents();
   grid_dependency_wait();
-  const int h = blockIdx.x, t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = a.heads / a.cache.kv_heads, kvh = h / R;
-  int b = t, keys;
-  if (DECODE) {
-    keys = a.ctx[t];
-  } else {
-    int hi = a.batch;                              // cu[b] <= t < cu[b + 1]
-    for (b = 0; hi - b > 1;) {
-      const int mid = (b + hi) / 2;
-      if (a.cu[mid] <= t) b = mid; else hi = mid;
-    }
-    keys = a.pos0[b] + t - a.cu[b] + 1;
+  cg::cluster_group cl = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, csize = gridDim.x / a.parts, rank = blockIdx.x % csize;
+  const int kvh = blockIdx.y / a.groups, group = blockIdx.y % a.groups, b = blockIdx.z;
+  const int R = a.heads / a.cache.kv_heads;
+  const int t_first = DECODE ? b : a.cu[b], n_tokens = DECODE ? 1 : a.cu[b + 1] - t_first;
+  if (!DECODE && n_tokens > 0 && (t_first < 0 || n_tokens > a.tokens - t_first)) {      // not rows of q
+    if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
+    return;
   }
-  uint16_t* out = a.out + ((int64_t)t * a.heads + h) * kDim;
-  const int64_t room = a.width * a.cache.block;
-  if (keys > room) { if (threadIdx.x == 0) report(a.status, NQB200_ERR_BAD_INDEX); keys = (int)room; }
-  if (keys <= 0) { out[threadIdx.x] = 0; return; }
-  if (DECODE) {
-    // half a warp a head: the query, the key, the value
-    const int l = threadIdx.x & 15, who = threadIdx.x >> 4;
-    const uint16_t* src = a.q + (int64_t)t * a.stride + (int64_t)(who == 0 ? h : who == 1 ? a.heads + kvh : a.heads + a.cache.kv_heads + kvh) * kDim;
-    float x[4], y[4], ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = raw16_to_float<BF16>(src[4 * l + e]);
-      y[e] = raw16_to_float<BF16>(src[64 + 4 * l + e]);
-      ss += x[e] * x[e] + y[e] * y[e];
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    int64_t pos = a.positions[t];
-    if (pos < 0 || pos >= a.max_positions) { if (threadIdx.x == 0) report(a.status, NQB200_ERR_BAD_INDEX); pos = 0; }
-    if (who < 2) {
-      const float inv = rsqrtf(ss / (float)kDim + a.eps);
-      const uint16_t* w = who ? a.kw : a.qw;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float u = x[e] * inv * raw16_to_float<BF16>(w[4 * l + e]), v = y[e] * inv * raw16_to_float<BF16>(w[64 + 4 * l + e]);
-        const float c = a.cos_sin[pos * kDim + 4 * l + e], s = a.cos_sin[pos * kDim + 64 + 4 * l + e];
-        x[e] = u * c - v * s;
-        y[e] = u * s + v * c;
-      }
-    }
-    if (who == 0) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { s_q[4 * l + e] = x[e]; s_q[64 + 4 * l + e] = y[e]; }
-    }
-    uint32_t word;
-    uint2 params;
-    quantise<BF16>(x, y, word, params);
-    if (who == 1 || who == 2) {
-      own[who - 1][l] = word;
-      if (l == 0) own_params[who - 1] = params;
-      const int64_t row = a.rows[t], page = row / a.cache.block;
-      if (h % R == 0 && row >= 0 && page < a.cache.pages) {
-        const int r = (int)(row - page * a.cache.block);
-        uint8_t* base = (who == 2 ? a.cache.v : a.cache.k) + page_at(a.cache, page, kvh);
-        reinterpret_cast<uint32_t*>(base + r * kData)[l] = word;
-        if (l == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
-      } else if (row >= 0 && page >= a.cache.pages && l == 0) {
-        report(a.status, NQB200_ERR_BAD_INDEX);
-      }
-    }
-  } else {
-    s_q[threadIdx.x] = raw16_to_float<BF16>(a.q[(int64_t)t * a.stride + (int64_t)h * kDim + threadIdx.x]);
+  const int cols = min(kCols, n_tokens * R - group * kCols);     // of this CTA
+  if (cols <= 0) return;                                         // the same for the whole cluster
+  const int first_pos = DECODE ? 0 : a.pos0[b];
+  // column c: row group * 8 + c of the sequence's (token, head of the group) rows
+  const auto token_of = [&](int c) { return (group * kCols + c) / R; };
+  int keys = DECODE ? a.ctx[b] : first_pos + token_of(cols - 1) + 1;
+  const int64_t room = (int64_t)a.width * a.cache.block;
+  if (keys > room || (!DECODE && (first_pos < 0 || n_tokens > a.max_len))) {
+    if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
+    keys = (int)min((int64_t)keys, room);
   }
-  __syncthreads();
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, sum = 0.f;
+  const int tiles = keys <= 0 ? 0 : (keys + kTile - 1) / kTile, per = (tiles + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int t0 = min((int)blockIdx.x * per, tiles), t1 = min(t0 + per, tiles);
+  const int stored = DECODE ? keys - 1 : keys;                   // keys that are read from the cache
+  const bool newest = DECODE && t1 == tiles && t0 < t1;          // this CTA has the tile with the step's own key
+  uint8_t* ring = smem + warp * (STAGES * kStage);
+  const uint32_t ring_a = smem_addr(ring);
+  const int32_t* table = a.table + (int64_t)b * a.width;
+
+  // 16-byte piece c of row r at r * 64 + (c ^ 2 bit 2 of r) * 16: eight lanes' pieces lie in different banks for keys (two rows that differ
+  // in their last bit) and for values (four rows, two of each parity, of which two have bit 2 set)
+  auto load = [&](int t, int stage) {
+    if (t < t1) {
+      const int p0 = t * kTile;
+      int64_t base[2];
+      int row0[2];
+      bool there[2];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) q[e] = s_q[4 * lane + e] * (a.scale * kLog2e);
-  for (int j = warp; j < keys; j += kWarps) {
-    float x[4], v[4];
-    if (DECODE && j == keys - 1) {
-      fetch<BF16>(own[0], own_params[0], x);
-      fetch<BF16>(own[1], own_params[1], v);
+      for (int h = 0; h < 2; ++h) {                // 16 rows lie in one page
+        if (h == 1 && a.cache.block % kTile == 0) { base[1] = base[0]; row0[1] = row0[0] + 16; there[1] = there[0] && p0 + 16 < stored; continue; }
+        const int key = p0 + 16 * h, at = (unsigned)key / (unsigned)a.cache.block;
+        there[h] = key < stored;
+        const int page = there[h] ? table[at] : 0;
+        if (page < 0 || page >= a.cache.pages) { there[h] = false; if (lane == 0) report(a.status, NQB200_ERR_BAD_INDEX); }
+        base[h] = there[h] ? page_at(a.cache, page, kvh) : 0;
+        row0[h] = key - at * a.cache.block;
+      }
+      const uint32_t dst = ring_a + stage * kStage;
+      const int c = lane & 3;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int h = i >> 1, r = i * 8 + (lane >> 2);
+        const int bytes = there[h] && p0 + r < stored ? 16 : 0;
+        const int64_t src = base[h] + (row0[h] + (r & 15)) * kData + c * 16;
+        const uint32_t to = dst + r * kData + ((c ^ ((r >> 1) & 2)) << 4);
+        copy16(to, a.cache.k + (bytes ? src : 0), bytes);
+        copy16(to + kOffV, a.cache.v + (bytes ? src : 0), bytes);
+      }
+      const int l = lane & 15;                     // parameters of rows 2 l and 2 l + 1, of keys and of values
+      const int left = (l < 8 ? there[0] : there[1]) ? stored - (p0 + 2 * l) : 0, bytes = left >= 2 ? 16 : left == 1 ? 8 : 0;
+      const int64_t src = bytes ? (l < 8 ? base[0] : base[1]) + (int64_t)a.cache.block * kData + ((l < 8 ? row0[0] : row0[1]) + 2 * (l & 7)) * kParams : 0;
+      copy16(dst + (lane < 16 ? kOffKP : kOffVP) + l * 16, (lane < 16 ? a.cache.k : a.cache.v) + src, bytes);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) load(t0 + warp + s * kWarps, s);
+
+  // queries into fx.q, zeros beyond `cols`: half a warp each
+  const int unit = tid >> 4, l16 = tid & 15;
+  if (DECODE) {
+    if (keys > 0) {
+      int64_t pos = a.positions[b];
+      if (pos < 0 || pos >= a.max_positions) {
+        if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
+        pos = 0;
+      }
+      const float* angles = a.cos_sin + pos * kDim;
+      const uint16_t* row = a.q + (int64_t)b * a.stride;
+      float x[4], y[4];
+      turned<BF16>(row + (int64_t)(kvh * R + group * kCols + min(unit, cols - 1)) * kDim, a.qw, angles, a.eps, x, y);
+      const bool in = unit < cols;
+      uint2* dst = reinterpret_cast<uint2*>(fx.q[unit]);
+      dst[l16] = in ? make_uint2(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])) : make_uint2(0u, 0u);
+      dst[l16 + 16] = in ? make_uint2(pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])) : make_uint2(0u, 0u);
+      if (newest && warp == 0) {                   // the key and the value
+        const bool is_v = unit == 1;
+        turned<BF16>(row + (int64_t)(a.heads + (is_v ? a.cache.kv_heads : 0) + kvh) * kDim, is_v ? nullptr : a.kw, angles, a.eps, x, y);
+        uint32_t word;
+        uint2 params;
+        quantise<BF16>(x, y, word, params);
+        fx.own[is_v][l16] = word;
+        if (l16 == 0) fx.own_params[is_v] = params;
+        const int64_t at = a.rows[b];
+        if (group == 0 && at >= 0) {
+          const int64_t page = at / a.cache.block;
+          if (page < a.cache.pages) {
+            const int r = (int)(at - page * a.cache.block);
+            uint8_t* base = (is_v ? a.cache.v : a.cache.k) + page_at(a.cache, page, kvh);
+            reinterpret_cast<uint32_t*>(base + r * kData)[l16] = word;
+            if (l16 == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
+          } else if (l16 == 0) {
+            report(a.status, NQB200_ERR_BAD_INDEX);
+          }
+        }
+      }
     } else {
-      const int page = a.table[(int64_t)b * a.width + j / a.cache.block], r = j % a.cache.block;
-      if (page < 0 || page >= a.cache.pages) { if (lane == 0) report(a.status, NQB200_ERR_BAD_INDEX); continue; }
-      const int64_t at = page_at(a.cache, page, kvh), par = at + (int64_t)a.cache.block * kData + r * kParams;
-      fetch<BF16>(reinterpret_cast<const uint32_t*>(a.cache.k + at + r * kData), *reinterpret_cast<const uint2*>(a.cache.k + par), x);
-      fetch<BF16>(reinterpret_cast<const uint32_t*>(a.cache.v + at + r * kData), *reinterpret_cast<const uint2*>(a.cache.v + par), v);
+      reinterpret_cast<uint4*>(fx.q[unit])[l16] = make_uint4(0u, 0u, 0u, 0u);
     }
-    float s = q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3];
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, k);
-    const float n = max_nan(m, s), f = exp2f(m - n), w = exp2f(s - n);
-    sum = sum * f + w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + w * v[e];
-    m = n;
+  } else {
+    const int idx = group * kCols + unit;
+    reinterpret_cast<uint4*>(fx.q[unit])[l16] =
+        unit < cols ? reinterpret_cast<const uint4*>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim)[l16] : make_uint4(0u, 0u, 0u, 0u);
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s_o[warp][4 * lane + e] = o[e];
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = sum; }
   __syncthreads();
-  float top = s_m[0], acc = 0.f, l = 0.f;
-  for (int w = 1; w < kWarps; ++w) top = max_nan(top, s_m[w]);
-  for (int w = 0; w < kWarps; ++w) {
-    const float f = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - top);
-    acc += f * s_o[w][threadIdx.x];
-    l += f * s_l[w];
+
+  const int g = lane >> 2, t4 = lane & 3;
+  // word j of a lane's 16 bytes of a key: dimensions 64 (j & 1) + 16 t4 + 8 (j >> 1) .. + 7
+  uint32_t qf[4][4];
+  float qs[2][2];                                  // [half][column 2 t4 + u]: sums of the query
+  {
+    float mine[2] = {0.f, 0.f};                    // of column g, over the lane's dimensions
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(&fx.q[g][64 * (j & 1) + 16 * t4 + 8 * (j >> 1)]);
+      qf[j][0] = v.x; qf[j][1] = v.y; qf[j][2] = v.z; qf[j][3] = v.w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[j & 1] += raw16_to_float<BF16>((uint16_t)(qf[j][i] & 0xFFFF)) + raw16_to_float<BF16>((uint16_t)(qf[j][i] >> 16));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mine[h] += __shfl_xor_sync(0xFFFFFFFFu, mine[h], 1);
+      mine[h] += __shfl_xor_sync(0xFFFFFFFFu, mine[h], 2);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) qs[h][u] = __shfl_sync(0xFFFFFFFFu, mine[h], (2 * t4 + u) * 4);
+    }
   }
-  out[threadIdx.x] = float_to_raw16<BF16>(l == 0.f ? 0.f : acc / l);
+  const float factor = a.scale * kLog2e;
+  // how many keys this lane's columns see, and the fewest of any column
+  int sees[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) sees[u] = DECODE ? keys : min(keys, first_pos + token_of(min(2 * t4 + u, cols - 1)) + 1);
+  const int all_see = DECODE ? keys : min(keys, first_pos + token_of(0) + 1);
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, L[2][2] = {{0.f, 0.f}, {0.f, 0.f}};     // L[half][column]: sums of weight times offset
+  float O[8][4], C[2][4];                          // O[4 half + i]: dimensions 64 half + 8 g + 2 i and + 1
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) O[i][e] = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) C[h][e] = 0.f;
+  float top_scale = 0.f, inv_scale = 0.f;          // float16: what the values' scales are relative to, a power of two, and its reciprocal
+  constexpr uint32_t kOnes = BF16 ? 0x3F803F80u : 0x3C003C00u;
+
+  // row i of a product's 16 keys is key i ^ bit 1 of i
+  const int key_g = g ^ ((g >> 1) & 1), kv0 = (2 * t4) ^ (t4 & 1), kv1 = (2 * t4 + 1) ^ (t4 & 1);
+  const int koff = key_g * kData + ((t4 ^ ((g >> 1) & 2)) << 4);
+  const int voff = kOffV + (((g >> 1) ^ (t4 & 2)) << 4) + (g & 1) * 8;
+
+  const auto tile = [&](auto edge, const uint8_t* st, int p0) {
+    constexpr bool EDGE = decltype(edge)::value;
+    float x[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {                  // 16 keys
+      const uint4 ka = *reinterpret_cast<const uint4*>(st + u * 16 * kData + koff), kb = *reinterpret_cast<const uint4*>(st + (u * 16 + 8) * kData + koff);
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mma<BF16>(c[j & 1], lift<BF16, 0>(wa[j]), lift<BF16, 0>(wb[j]), lift<BF16, 1>(wa[j]), lift<BF16, 1>(wb[j]), qf[j][0], qf[j][1]);
+        mma<BF16>(c[j & 1], lift<BF16, 2>(wa[j]), lift<BF16, 2>(wb[j]), lift<BF16, 3>(wa[j]), lift<BF16, 3>(wb[j]), qf[j][2], qf[j][3]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint2 p = *reinterpret_cast<const uint2*>(st + kOffKP + (u * 16 + 8 * r + key_g) * kParams);
+        const float s0 = 16.f * scale_of<BF16>(p.x), s1 = 16.f * scale_of<BF16>(p.y), o0 = offset_of<BF16>(p.x) - s0, o1 = offset_of<BF16>(p.y) - s1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          x[u][2 * r + h] = (fmaf(s0, c[0][2 * r + h], s1 * c[1][2 * r + h]) + fmaf(o0, qs[0][h], o1 * qs[1][h])) * factor;
+      }
+    }
+    const auto seen = [&](int u, int e) { return !EDGE || p0 + u * 16 + 8 * (e >> 1) + key_g < sees[e & 1]; };
+    if (EDGE) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[u][e] = seen(u, e) ? x[u][e] : -INFINITY;
+    }
+    uint2 vp[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) vp[u][r] = *reinterpret_cast<const uint2*>(st + kOffVP + (u * 16 + 8 * r + key_g) * kParams);
+    float top[2] = {fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]))};
+    float far[2] = {1.f, 1.f};                     // what the sums so far are multiplied by
+    bool moves = top[0] > m[0] + kLag || top[1] > m[1] + kLag;
+    float s_top = 0.f;
+    if (!BF16) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s0 = scale_of<BF16>(vp[u][r].x), s1 = scale_of<BF16>(vp[u][r].y);
+          s_top = fmaxf(s_top, fmaxf(s0 < INFINITY ? s0 : 0.f, s1 < INFINITY ? s1 : 0.f));     // (not a NaN either)
+        }
+      moves = moves || s_top > top_scale;
+    }
+    if (__any_sync(0xFFFFFFFFu, moves)) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
+        top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], o));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float n = fmaxf(m[h], top[h]);
+        far[h] = m[h] == n ? 1.f : exp2_fast(m[h] - n);      // 0 ahead of the first tile
+        m[h] = n;
+        l[h] *= far[h];
+        L[0][h] *= far[h];
+        L[1][h] *= far[h];
+      }
+      float same = 1.f;
+      if (!BF16) {
+        const float s_all = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(s_top)));
+        if (s_all > top_scale) {                   // twice the next power of two
+          const float n = __uint_as_float((__float_as_uint(s_all) & 0x7F800000u) + 0x01000000u);
+          same = top_scale / n;
+          top_scale = n;
+          inv_scale = 1.f / n;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[i][e] *= far[e & 1] * same;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) C[h][e] *= far[e & 1] * same;
+    }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    uint32_t w[2][2][2];                           // [16 keys][half][rows of 8]: weights as the second operand
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float p[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { p[h] = exp2_fast(x[u][2 * r + h] - ref[h]); l[h] += p[h]; }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t par = half ? vp[u][r].y : vp[u][r].x;
+          const float s = BF16 ? scale_of<BF16>(par) : scale_of<BF16>(par) * inv_scale, o = offset_of<BF16>(par);
+          // a key that a column does not see has no part in it, even where its value is not a number
+          if (EDGE) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) L[half][h] = seen(u, 2 * r + h) ? fmaf(p[h], o, L[half][h]) : L[half][h];
+            w[u][half][r] = transpose8(pack2<BF16>(seen(u, 2 * r) ? p[0] * s : 0.f, seen(u, 2 * r + 1) ? p[1] * s : 0.f));
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) L[half][h] = fmaf(p[h], o, L[half][h]);
+            w[u][half][r] = transpose8(pack2<BF16>(p[0] * s, p[1] * s));
+          }
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* vs = st + u * 16 * kData + voff;
+      const uint2 va = *reinterpret_cast<const uint2*>(vs + kv0 * kData), vb = *reinterpret_cast<const uint2*>(vs + kv1 * kData);
+      const uint2 vc = *reinterpret_cast<const uint2*>(vs + (kv0 + 8) * kData), vd = *reinterpret_cast<const uint2*>(vs + (kv1 + 8) * kData);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t a_ = half ? va.y : va.x, b_ = half ? vb.y : vb.x, c_ = half ? vc.y : vc.x, d_ = half ? vd.y : vd.x;
+        // dimensions of the word's low and high 16 bits, of two keys each
+        const uint32_t lo0 = __byte_perm(a_, b_, 0x5410), hi0 = __byte_perm(a_, b_, 0x7632), lo1 = __byte_perm(c_, d_, 0x5410), hi1 = __byte_perm(c_, d_, 0x7632);
+        const uint32_t b0 = w[u][half][0], b1 = w[u][half][1];
+        mma<BF16>(O[4 * half], lift<BF16, 0>(lo0), lift<BF16, 0>(hi0), lift<BF16, 0>(lo1), lift<BF16, 0>(hi1), b0, b1);
+        mma<BF16>(O[4 * half + 1], lift<BF16, 1>(lo0), lift<BF16, 1>(hi0), lift<BF16, 1>(lo1), lift<BF16, 1>(hi1), b0, b1);
+        mma<BF16>(O[4 * half + 2], lift<BF16, 2>(lo0), lift<BF16, 2>(hi0), lift<BF16, 2>(lo1), lift<BF16, 2>(hi1), b0, b1);
+        mma<BF16>(O[4 * half + 3], lift<BF16, 3>(lo0), lift<BF16, 3>(hi0), lift<BF16, 3>(lo1), lift<BF16, 3>(hi1), b0, b1);
+        mma<BF16>(C[half], kOnes, kOnes, kOnes, kOnes, b0, b1);
+      }
+    }
+  };
+
+  int stage = 0;
+  for (int t = t0 + warp; t < t1; t += kWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();                                  // the tile is there for every lane, the one before it is no longer read
+    load(t + (STAGES - 1) * kWarps, stage == 0 ? STAGES - 1 : stage - 1);
+    uint8_t* st = ring + stage * kStage;
+    const int p0 = t * kTile;
+    if (DECODE && t == tiles - 1) {                // the step's own key and value go into the tile
+      const int r = keys - 1 - p0, c = lane & 15, which = lane >> 4;
+      reinterpret_cast<uint32_t*>(st + (which ? kOffV : 0) + r * kData + (((c >> 2) ^ ((r >> 1) & 2)) << 4))[c & 3] = fx.own[which][c];
+      if (c == 0) *reinterpret_cast<uint2*>(st + (which ? kOffVP : kOffKP) + r * kParams) = fx.own_params[which];
+      __syncwarp();
+    }
+    if (p0 + kTile > all_see) tile(std::true_type(), st, p0); else tile(std::false_type(), st, p0);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+
+  // the warps' shares over their rings
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], o);
+      L[0][h] += __shfl_xor_sync(0xFFFFFFFFu, L[0][h], o);
+      L[1][h] += __shfl_xor_sync(0xFFFFFFFFu, L[1][h], o);
+    }
+  }
+  float* po = reinterpret_cast<float*>(ring);      // [column][kOS]
+  const float unit_scale = BF16 ? 16.f : 16.f * top_scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int half = i >> 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 v = make_float2(fmaf(O[i][h] - C[half][h], unit_scale, L[half][h]), fmaf(O[i][2 + h] - C[half][h], unit_scale, L[half][h]));
+      *reinterpret_cast<float2*>(po + (2 * t4 + h) * kOS + 64 * half + 8 * g + 2 * (i & 3)) = v;
+    }
+  }
+  if (lane < 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) { fx.m[warp][2 * lane + h] = m[h]; fx.l[warp][2 * lane + h] = l[h]; }
+  }
+  __syncthreads();
+  const auto finish = [&](int c, int d, float o, float sum, float top) {
+    const int idx = group * kCols + c;
+    const int64_t row = (int64_t)(t_first + idx / R) * a.heads + kvh * R + idx % R;
+    if (a.parts > 1) {
+      float* share = a.shares + (row * a.parts + blockIdx.x / csize) * kShare;
+      share[d] = o;
+      if (d == 0) { share[kDim] = top; share[kDim + 1] = sum; }
+    } else {
+      a.out[row * kDim + d] = float_to_raw16<BF16>(sum == 0.f ? 0.f : o / sum);
+    }
+  };
+  for (int c = 0; c < cols; ++c) {
+    float top = -INFINITY, o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, fx.m[w][c]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = fx.m[w][c] == top ? 1.f : exp2_fast(fx.m[w][c] - top);      // 0: a warp without keys
+      o += f * reinterpret_cast<const float*>(smem + w * (STAGES * kStage))[c * kOS + tid];
+      sum += f * fx.l[w][c];
+    }
+    if (csize == 1) {
+      finish(c, tid, o, sum, top);
+    } else {
+      fx.out[c][tid] = o;
+      if (tid == 0) { fx.cm[c] = top; fx.cl[c] = sum; }
+    }
+  }
+  if (csize == 1) return;
+  cl.sync();
+  for (int e = rank * kThreads + tid; e < cols * kDim; e += csize * kThreads) {
+    const int c = e / kDim, d = e % kDim;
+    float pm[8], pl[8], po8[8], top = -INFINITY, o = 0.f, sum = 0.f;              // all of the cluster's shares at once
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const Fixed* s = cl.map_shared_rank(&fx, k < csize ? k : 0);
+      pm[k] = k < csize ? s->cm[c] : -INFINITY;
+      pl[k] = s->cl[c];
+      po8[k] = s->out[c][d];
+      top = fmaxf(top, pm[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = k >= csize ? 0.f : pm[k] == top ? 1.f : exp2_fast(pm[k] - top);
+      o += f * po8[k];
+      sum += f * pl[k];
+    }
+    finish(c, d, o, sum, top);
+  }
+  cl.sync();                                       // peers may still read this CTA's shared memory
 }
 
-template <bool DECODE> int launch(const Args& a, int64_t tokens, int dtype, cudaStream_t st) {
-  return launch_overlapped(dtype == NQB200_BF16 ? kv4_rows_kernel<true, DECODE> : kv4_rows_kernel<false, DECODE>, dim3((unsigned)a.heads, (unsigned)tokens),
-                           dim3(32 * kWarps), 0, st, a);
+// The shares of a row's clusters, a CTA per (token, query head), in the clusters' order.
+template <bool BF16>
+__global__ void __launch_bounds__(kDim) kv4_shares_kernel(const float* __restrict__ shares, uint16_t* __restrict__ out, int parts) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int64_t row = blockIdx.x;
+  const float* s = shares + row * parts * kShare;
+  float top = -INFINITY, sum = 0.f, o = 0.f;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, s[p * kShare + kDim]);
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float m = s[p * kShare + kDim], f = m == top ? 1.f : exp2f(m - top);
+    o += f * s[p * kShare + threadIdx.x];
+    sum += f * s[p * kShare + kDim + 1];
+  }
+  out[row * kDim + threadIdx.x] = float_to_raw16<BF16>(sum == 0.f ? 0.f : o / sum);
 }
+
+// How a call is split: CTAs of a cluster, clusters of a sequence, tiles of a warp's ring.
+constexpr int kResident[4][2] = {{296, 592}, {148, 296}, {71, 142}, {33, 66}};   // clusters of 1, 2, 4, 8 CTAs that are resident with rings of 4 and 2 tiles
+constexpr int kMostParts = 16;
+struct Split { int csize, stages, parts; };
+Split split(int64_t units, int64_t keys) {
+  Split s = {1, 2, 1};
+  int row = 0;
+  while (row < 3 && units <= kResident[row + 1][1] && keys > (int64_t)s.csize * kWarps * kTile) { s.csize *= 2; ++row; }
+  if (row == 3 && keys >= 8 * 1024)
+    while (s.parts < kMostParts && units * s.parts * 2 <= kResident[3][1] && keys >= 8 * s.parts * 2 * 256) s.parts *= 2;
+  if (units * s.parts <= kResident[row][0]) s.stages = 4;
+  return s;
+}
+
+int groups_of(int64_t tokens, int64_t heads, int64_t kv_heads) { return (int)((tokens * (heads / kv_heads) + kCols - 1) / kCols); }
+
+template <bool BF16, bool DECODE, int STAGES> int launch_stages(const Args& a, int csize, int64_t batch, cudaStream_t st) {
+  const auto kernel = kv4_rows_kernel<BF16, DECODE, STAGES>;
+  constexpr int smem = smem_bytes(STAGES);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) { cudaGetLastError(); return NQB200_ERR_LAUNCH; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(csize * a.parts), (unsigned)(a.cache.kv_heads * a.groups), (unsigned)batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)csize;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { cudaGetLastError(); return NQB200_ERR_LAUNCH; }
+  return NQB200_OK;
+}
+template <bool BF16, bool DECODE> int launch_t(Args& a, int64_t batch, int64_t tokens, int64_t keys, cudaStream_t st) {
+  const Split s = split((int64_t)a.cache.kv_heads * a.groups * batch, keys);
+  a.parts = s.parts;
+  const int rc = s.stages == 4 ? launch_stages<BF16, DECODE, 4>(a, s.csize, batch, st) : launch_stages<BF16, DECODE, 2>(a, s.csize, batch, st);
+  if (rc != NQB200_OK || s.parts == 1) return rc;
+  return launch_overlapped(kv4_shares_kernel<BF16>, dim3((unsigned)(tokens * a.heads)), dim3(kDim), 0, st, (const float*)a.shares, a.out, s.parts);
+}
+template <bool DECODE> int launch(Args& a, int64_t batch, int64_t tokens, int64_t keys, int dtype, cudaStream_t st) {
+  return dtype == NQB200_BF16 ? launch_t<true, DECODE>(a, batch, tokens, keys, st) : launch_t<false, DECODE>(a, batch, tokens, keys, st);
+}
+size_t scratch_bytes_of(int64_t batch, int64_t tokens, int64_t max_len, int64_t keys, int64_t heads, int64_t kv_heads) {
+  const Split s = split(kv_heads * groups_of(max_len, heads, kv_heads) * batch, keys);
+  return s.parts > 1 ? (size_t)(tokens * heads * s.parts * kShare) * sizeof(float) : 0;
+}
+bool heads_fit(int64_t heads, int64_t kv_heads) { return kv_heads > 0 && kv_heads <= 4096 && heads > 0 && heads <= 65535 && heads % kv_heads == 0; }
+bool table_fits(int64_t width, int64_t block) { return width > 0 && block > 0 && width <= INT32_MAX / block; }
 
 }  // namespace
 }  // namespace nqb200
@@ -157,44 +597,61 @@ using namespace nqb200;
 static int check_heads(const nqb200_kv4* cache, int64_t heads, int64_t width, int dtype) {
   const int rc = kv4::check_cache(cache);
   if (rc != NQB200_OK) return rc;
-  if (heads <= 0 || heads > 65535 || heads % cache->kv_heads != 0 || width <= 0 || width > INT32_MAX) return NQB200_ERR_BAD_SHAPE;
+  if (!heads_fit(heads, cache->kv_heads) || !table_fits(width, cache->block_size)) return NQB200_ERR_BAD_SHAPE;
   return dtype == NQB200_F16 || dtype == NQB200_BF16 ? NQB200_OK : NQB200_ERR_BAD_DTYPE;
 }
 
-extern "C" size_t nqb200_kv4_decode_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t nqb200_kv4_decode_scratch_bytes(int64_t table_width, int64_t block_size, int64_t batch, int64_t num_q_heads, int64_t kv_heads) {
+  if (!heads_fit(num_q_heads, kv_heads) || !table_fits(table_width, block_size) || batch <= 0 || batch > 65535) return 0;
+  return scratch_bytes_of(batch, batch, 1, table_width * block_size, num_q_heads, kv_heads);
+}
 
 extern "C" int nqb200_kv4_decode_attention(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
                                            int64_t max_positions, const int64_t* positions, const int64_t* rows, const nqb200_kv4* cache,
                                            const int32_t* table, int64_t table_width, const int32_t* ctx, void* out, int64_t batch, int64_t num_q_heads,
-                                           float scale, float eps, int dtype, void*, size_t, int* status, void* stream) {
+                                           float scale, float eps, int dtype, void* scratch, size_t scratch_bytes, int* status, void* stream) {
   const int rc = check_heads(cache, num_q_heads, table_width, dtype);
   if (rc != NQB200_OK) return rc;
-  if (batch < 0 || batch > 65535 || max_positions <= 0 || row_stride < (num_q_heads + 2 * cache->kv_heads) * kv4::kDim || row_stride % 8 != 0) return NQB200_ERR_BAD_SHAPE;
+  const int groups = groups_of(1, num_q_heads, cache->kv_heads);
+  if (batch < 0 || batch > 65535 || cache->kv_heads * groups > 65535 || max_positions <= 0 || row_stride < (num_q_heads + 2 * cache->kv_heads) * kv4::kDim || row_stride % 8 != 0)
+    return NQB200_ERR_BAD_SHAPE;
   if (batch == 0) return NQB200_OK;
   if (!qkv || !q_weight || !k_weight || !cos_sin || !positions || !rows || !table || !ctx || !out) return NQB200_ERR_NULL_POINTER;
-  if (!aligned16(qkv) || !aligned16(out)) return NQB200_ERR_MISALIGNED;
+  if (!aligned16(qkv) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos_sin) || !aligned16(out)) return NQB200_ERR_MISALIGNED;
+  const size_t need = nqb200_kv4_decode_scratch_bytes(table_width, cache->block_size, batch, num_q_heads, cache->kv_heads);
+  if (need > 0 && (!scratch || scratch_bytes < need)) return NQB200_ERR_WORKSPACE;
+  if (need > 0 && !aligned16(scratch)) return NQB200_ERR_MISALIGNED;
   Args a = {};
   a.q = (const uint16_t*)qkv; a.stride = row_stride; a.qw = (const uint16_t*)q_weight; a.kw = (const uint16_t*)k_weight;
   a.cos_sin = cos_sin; a.max_positions = max_positions; a.positions = positions; a.rows = rows; a.cache = kv4::cache_of(cache);
-  a.table = table; a.width = table_width; a.ctx = ctx; a.out = (uint16_t*)out; a.batch = (int)batch; a.heads = (int)num_q_heads;
-  a.scale = scale; a.eps = eps; a.status = status;
-  return launch<true>(a, batch, dtype, (cudaStream_t)stream);
+  a.table = table; a.width = (int)table_width; a.ctx = ctx; a.out = (uint16_t*)out; a.heads = (int)num_q_heads; a.groups = groups; a.max_len = 1;
+  a.scale = scale; a.eps = eps; a.status = status; a.shares = (float*)scratch;
+  return launch<true>(a, batch, batch, table_width * cache->block_size, dtype, (cudaStream_t)stream);
 }
 
-extern "C" size_t nqb200_kv4_prompt_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads, int64_t kv_heads) {
+  if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || batch > 65535 || T <= 0 || max_len <= 0 || max_ctx < max_len) return 0;
+  return scratch_bytes_of(batch, T, max_len, max_ctx, num_q_heads, kv_heads);
+}
 
 extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, const nqb200_kv4* cache, const int32_t* table, int64_t table_width,
                                            const int32_t* cu, const int32_t* pos0, void* out, int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx,
-                                           int64_t tiles, int64_t num_q_heads, float scale, int dtype, void*, size_t, int* status, void* stream) {
+                                           int64_t tiles, int64_t num_q_heads, float scale, int dtype, void* scratch, size_t scratch_bytes, int* status, void* stream) {
   const int rc = check_heads(cache, num_q_heads, table_width, dtype);
   if (rc != NQB200_OK) return rc;
-  if (batch < 0 || batch > 65535 || T < 0 || T > 65535 || max_len < 0 || max_ctx < max_len || tiles < 0 || q_stride < num_q_heads * kv4::kDim || q_stride % 8 != 0)
+  if (batch < 0 || batch > 65535 || T < 0 || T > INT32_MAX / num_q_heads || max_len < 0 || (T > 0 && max_len > T) || max_ctx < max_len || max_ctx > INT32_MAX || tiles < 0 ||
+      q_stride < num_q_heads * kv4::kDim || q_stride % 8 != 0)
     return NQB200_ERR_BAD_SHAPE;
   if (batch == 0 || T == 0) return NQB200_OK;
+  const int64_t groups = groups_of(max_len, num_q_heads, cache->kv_heads);
+  if (max_len == 0 || cache->kv_heads * groups > 65535) return NQB200_ERR_BAD_SHAPE;
   if (!q || !table || !cu || !pos0 || !out) return NQB200_ERR_NULL_POINTER;
   if (!aligned16(q) || !aligned16(out)) return NQB200_ERR_MISALIGNED;
+  const size_t need = nqb200_kv4_prompt_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);
+  if (need > 0 && (!scratch || scratch_bytes < need)) return NQB200_ERR_WORKSPACE;
+  if (need > 0 && !aligned16(scratch)) return NQB200_ERR_MISALIGNED;
   Args a = {};
-  a.q = (const uint16_t*)q; a.stride = q_stride; a.cache = kv4::cache_of(cache); a.table = table; a.width = table_width; a.cu = cu; a.pos0 = pos0;
-  a.out = (uint16_t*)out; a.batch = (int)batch; a.heads = (int)num_q_heads; a.max_len = (int)max_len; a.max_ctx = (int)max_ctx; a.scale = scale; a.status = status;
-  return launch<false>(a, T, dtype, (cudaStream_t)stream);
+  a.q = (const uint16_t*)q; a.stride = q_stride; a.cache = kv4::cache_of(cache); a.table = table; a.width = (int)table_width; a.cu = cu; a.pos0 = pos0;
+  a.out = (uint16_t*)out; a.heads = (int)num_q_heads; a.groups = (int)groups; a.tokens = (int)T; a.max_len = (int)max_len; a.scale = scale; a.status = status; a.shares = (float*)scratch;
+  return launch<false>(a, batch, T, max_ctx, dtype, (cudaStream_t)stream);
 }

@@ -8,7 +8,7 @@ r is row ``r % block_size`` of page ``r // block_size``, as for the 16-bit cache
 The reference has no cache; what the store and the decode step compute ahead of it is its QK-norm and rotary embedding
 (nanoquantization/models/qwen3_quantized.py:88, layers/rope.py:24-45), here in 32 bits and rounded once.
 
-A page, cache row or position outside its buffer is never followed: the kernels leave it out and record it, and
+A page, cache row or position outside its buffer is never followed: the kernels take zeros in its place and record it, and
 ``_lib.check_cache_status()`` (the engine calls it after every step) raises."""
 from __future__ import annotations
 
