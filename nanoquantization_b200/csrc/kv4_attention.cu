@@ -6,17 +6,20 @@
 // take tiles of 32 keys on their own, through rings that they fill with cp.async.  Both products are mma m16n8k16 with the columns as the
 // eight columns of its result:
 //
-//   numbers  a nibble n becomes 1 + n/16, one shift and one logical operation for a pair: the nibble goes into the mantissa of 1.
-//            Nothing is subtracted and nothing scaled before a product.  With S = 16 scale and T = offset - S a value is S (1 + n/16) + T.
-//   scores   per group of 64 dimensions the product c of the lifted key and the query, then score = S0 c0 + S1 c1 + T0 q0 + T1 q1,
-//            q0 and q1 the sums of the query's halves, all in float.  Keys are exact; the query is the only thing that is rounded.
-//   values   the weight times the value's scale goes into the product, rounded once, a version for each of the two groups; the product
-//            with a matrix of ones gives the sum of just these rounded weights, and 16 (product - sum) + sum(weight offset) is the result.
-//            With float16 the scales are taken relative to the largest that the warp has seen, so that tiny values keep their bits.
+//   numbers  a nibble n becomes 1024 + n or 1024 + 16 n, a pair of them by one logical operation: it goes into the mantissa of float16's
+//            1024, one shift for a word of eight.  float16 operands and float accumulators serve both types.
+//   scores   per group of 64 dimensions the product of these numbers and the query (which has the sixteenths in it), whose accumulator starts
+//            at minus 1024 times the query's sum; score = f (s0 c0 + s1 c1) + m0 q0 + m1 q1 with the key's scales and offsets and the
+//            sums of the query's halves, in float.  Keys are exact; the query is rounded to float16 relative to its largest element, a
+//            power of two of its own.
+//   values   n - 8 by a packed operation more: over thousands of keys a sum with 1024 in it loses what the tensor cores cut off it (1500 keys:
+//            0.0022 off), and so does, less, one of numbers above 0.  The weight times the value's scale goes into the product, a version for each
+//            of the two groups, rounded to float16 once; scales are taken relative to the largest that the warp has seen, so that
+//            any type's values keep their bits.  What the level 8 stands for is summed in float.
 //   order    a lane owns 16 neighbouring bytes of a key and 8 of a value, which one load fetches; which dimension is which row of a
 //            product follows from that, as the layout of a row was chosen.
 //
-// The running maximum of a column moves only when a score is 8 (in log2 units) above it, found by one vote per 32 keys.  The warps meet in
+// Scores come out relative to a reference, which moves only when one is 8 (in log2 units) above it, found by one vote per 32 keys.  The warps meet in
 // shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
 #include <cooperative_groups.h>
 #include <type_traits>
@@ -57,6 +60,7 @@ struct Fixed {                                    // behind the rings
   uint2 own_params[2];
   float m[kWarps][kCols], l[kWarps][kCols];
   float cm[kCols], cl[kCols];                     // of the CTA, read by the cluster
+  float unit[kCols];                              // of the queries
   float out[kCols][kDim];
 };
 __host__ __device__ constexpr int ring_bytes(int stages) { return kWarps * stages * kStage; }
@@ -66,14 +70,9 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {      // zeros behind `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
 }
-template <bool BF16>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -82,16 +81,45 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// Nibbles I and I + 4 of a word as 1 + n/16 in both halves.
-template <bool BF16, int I> __device__ __forceinline__ uint32_t lift(uint32_t w) {
-  constexpr int to = BF16 ? 3 - 4 * I : 6 - 4 * I;
-  const uint32_t x = to > 0 ? w << (to > 0 ? to : 0) : w >> (to > 0 ? 0 : -to);
-  return BF16 ? (x & 0x00780078u) | 0x3F803F80u : (x & 0x03C003C0u) | 0x3C003C00u;
+// Nibbles I and I + 4 of a word, as pairs of float16: 1024 + n for even I, 1024 + 16 n for odd I.  `magic` is a pair of 1024 in a register:
+// with two immediate operands it would be two instructions.
+struct Lifted { uint32_t v[4]; };
+__device__ __forceinline__ Lifted lift(uint32_t w, uint32_t magic) {
+  const uint32_t x = w >> 8;
+  Lifted r;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r.v[0]) : "r"(w), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r.v[1]) : "r"(w), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r.v[2]) : "r"(x), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r.v[3]) : "r"(x), "r"(magic));
+  return r;
 }
-template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if (BF16) { const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&v); }
+// The same as n - 8.
+__device__ __forceinline__ Lifted levels(uint32_t w, uint32_t magic) {
+  Lifted r = lift(w, magic);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2& v = *reinterpret_cast<__half2*>(&r.v[i]);
+    v = i & 1 ? __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hadd2(v, __float2half2_rn(-1032.f));
+  }
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// A query as the first product's second operand, in units of a power of two that puts its largest element between 256 and 512: half a
+// warp, as for turned(); elements that meet 1024 + 16 n are divided by 16.  Returns the unit.
+__device__ __forceinline__ float operand(const float (&x)[4], const float (&y)[4], uint2& lo, uint2& hi) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  const uint32_t e = min(max(__float_as_uint(top) >> 23, 9u), 253u);
+  const float f = __uint_as_float((262u - e) << 23), f16 = f * 0.0625f;
+  lo = make_uint2(pack2(x[0] * f, x[1] * f), pack2(x[2] * f16, x[3] * f16));       // dimensions 4 l .. 4 l + 3: lifted pairs of even and odd number
+  hi = make_uint2(pack2(y[0] * f, y[1] * f), pack2(y[2] * f16, y[3] * f16));
+  return __uint_as_float((e - 8u) << 23);
 }
 
 // A head after norm and rotation: half a warp, lane l has dimensions 4 l .. and 64 + 4 l ..; `weight` null: as it is.
@@ -199,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load(t0 + warp + s * kWarps, s);
 
-  // queries into fx.q, zeros beyond `cols`: half a warp each
+  // queries into fx.q: half a warp each
   const int unit = tid >> 4, l16 = tid & 15;
   if (DECODE) {
     if (keys > 0) {
@@ -212,10 +240,11 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
       const uint16_t* row = a.q + (int64_t)b * a.stride;
       float x[4], y[4];
       turned<BF16>(row + (int64_t)(kvh * R + group * kCols + min(unit, cols - 1)) * kDim, a.qw, angles, a.eps, x, y);
-      const bool in = unit < cols;
-      uint2* dst = reinterpret_cast<uint2*>(fx.q[unit]);
-      dst[l16] = in ? make_uint2(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])) : make_uint2(0u, 0u);
-      dst[l16 + 16] = in ? make_uint2(pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])) : make_uint2(0u, 0u);
+      uint2 lo, hi;
+      const float f = operand(x, y, lo, hi);       // (columns beyond `cols` repeat the last one and are not used)
+      reinterpret_cast<uint2*>(fx.q[unit])[l16] = lo;
+      reinterpret_cast<uint2*>(fx.q[unit])[l16 + 16] = hi;
+      if (l16 == 0) fx.unit[unit] = f;
       if (newest && warp == 0) {                   // the key and the value
         const bool is_v = unit == 1;
         turned<BF16>(row + (int64_t)(a.heads + (is_v ? a.cache.kv_heads : 0) + kvh) * kDim, is_v ? nullptr : a.kw, angles, a.eps, x, y);
@@ -237,56 +266,68 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
           }
         }
       }
-    } else {
-      reinterpret_cast<uint4*>(fx.q[unit])[l16] = make_uint4(0u, 0u, 0u, 0u);
     }
   } else {
-    const int idx = group * kCols + unit;
-    reinterpret_cast<uint4*>(fx.q[unit])[l16] =
-        unit < cols ? reinterpret_cast<const uint4*>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim)[l16] : make_uint4(0u, 0u, 0u, 0u);
+    const int idx = group * kCols + min(unit, cols - 1);
+    float x[4], y[4];
+    turned<BF16>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim, nullptr, nullptr, 0.f, x, y);
+    uint2 lo, hi;
+    const float f = operand(x, y, lo, hi);
+    reinterpret_cast<uint2*>(fx.q[unit])[l16] = lo;
+    reinterpret_cast<uint2*>(fx.q[unit])[l16 + 16] = hi;
+    if (l16 == 0) fx.unit[unit] = f;
   }
   __syncthreads();
 
   const int g = lane >> 2, t4 = lane & 3;
   // word j of a lane's 16 bytes of a key: dimensions 64 (j & 1) + 16 t4 + 8 (j >> 1) .. + 7
   uint32_t qf[4][4];
-  float qs[2][2];                                  // [half][column 2 t4 + u]: sums of the query
+  // of columns 2 t4 + u: the unit of scores in log2 units, the sums of the query's halves in it, and minus 1024 times the operand's sums
+  float f[2], qs[2][2], start[2][2];
   {
-    float mine[2] = {0.f, 0.f};                    // of column g, over the lane's dimensions
+    float even[2] = {0.f, 0.f}, odd[2] = {0.f, 0.f};       // of column g, over the lane's dimensions
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint4 v = *reinterpret_cast<const uint4*>(&fx.q[g][64 * (j & 1) + 16 * t4 + 8 * (j >> 1)]);
       qf[j][0] = v.x; qf[j][1] = v.y; qf[j][2] = v.z; qf[j][3] = v.w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[j & 1] += raw16_to_float<BF16>((uint16_t)(qf[j][i] & 0xFFFF)) + raw16_to_float<BF16>((uint16_t)(qf[j][i] >> 16));
+      for (int i = 0; i < 4; ++i) {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&qf[j][i]));
+        (i & 1 ? odd : even)[j & 1] += p.x + p.y;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) f[u] = a.scale * kLog2e * fx.unit[2 * t4 + u];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      mine[h] += __shfl_xor_sync(0xFFFFFFFFu, mine[h], 1);
-      mine[h] += __shfl_xor_sync(0xFFFFFFFFu, mine[h], 2);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) qs[h][u] = __shfl_sync(0xFFFFFFFFu, mine[h], (2 * t4 + u) * 4);
+      for (int o = 1; o < 4; o <<= 1) {
+        even[h] += __shfl_xor_sync(0xFFFFFFFFu, even[h], o);
+        odd[h] += __shfl_xor_sync(0xFFFFFFFFu, odd[h], o);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float p = __shfl_sync(0xFFFFFFFFu, even[h], (2 * t4 + u) * 4), q = __shfl_sync(0xFFFFFFFFu, odd[h], (2 * t4 + u) * 4);
+        qs[h][u] = f[u] * fmaf(16.f, q, p);
+        start[h][u] = -1024.f * (p + q);
+      }
     }
   }
-  const float factor = a.scale * kLog2e;
+  uint32_t magic;                                  // (out of the compiler's sight, see lift)
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
   // how many keys this lane's columns see, and the fewest of any column
   int sees[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) sees[u] = DECODE ? keys : min(keys, first_pos + token_of(min(2 * t4 + u, cols - 1)) + 1);
   const int all_see = DECODE ? keys : min(keys, first_pos + token_of(0) + 1);
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, L[2][2] = {{0.f, 0.f}, {0.f, 0.f}};     // L[half][column]: sums of weight times offset
-  float O[8][4], C[2][4];                          // O[4 half + i]: dimensions 64 half + 8 g + 2 i and + 1
+  float m[2] = {-INFINITY, -INFINITY}, ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, L[2][2] = {{0.f, 0.f}, {0.f, 0.f}};     // L[half][column]: sums of weight times level 8
+  float O[8][4];                                   // O[4 half + i]: dimensions 64 half + 8 g + 2 i and + 1
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) O[i][e] = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) C[h][e] = 0.f;
-  float top_scale = 0.f, inv_scale = 0.f;          // float16: what the values' scales are relative to, a power of two, and its reciprocal
-  constexpr uint32_t kOnes = BF16 ? 0x3F803F80u : 0x3C003C00u;
+  float top_scale = 0.f, inv_scale = 0.f;          // what the values' scales are relative to, a power of two, and its reciprocal
 
   // row i of a product's 16 keys is key i ^ bit 1 of i
   const int key_g = g ^ ((g >> 1) & 1), kv0 = (2 * t4) ^ (t4 & 1), kv1 = (2 * t4 + 1) ^ (t4 & 1);
@@ -300,19 +341,20 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
     for (int u = 0; u < 2; ++u) {                  // 16 keys
       const uint4 ka = *reinterpret_cast<const uint4*>(st + u * 16 * kData + koff), kb = *reinterpret_cast<const uint4*>(st + (u * 16 + 8) * kData + koff);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float c[2][4] = {{start[0][0], start[0][1], start[0][0], start[0][1]}, {start[1][0], start[1][1], start[1][0], start[1][1]}};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        mma<BF16>(c[j & 1], lift<BF16, 0>(wa[j]), lift<BF16, 0>(wb[j]), lift<BF16, 1>(wa[j]), lift<BF16, 1>(wb[j]), qf[j][0], qf[j][1]);
-        mma<BF16>(c[j & 1], lift<BF16, 2>(wa[j]), lift<BF16, 2>(wb[j]), lift<BF16, 3>(wa[j]), lift<BF16, 3>(wb[j]), qf[j][2], qf[j][3]);
+        const Lifted la = lift(wa[j], magic), lb = lift(wb[j], magic);
+        mma(c[j & 1], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
+        mma(c[j & 1], la.v[2], lb.v[2], la.v[3], lb.v[3], qf[j][2], qf[j][3]);
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint2 p = *reinterpret_cast<const uint2*>(st + kOffKP + (u * 16 + 8 * r + key_g) * kParams);
-        const float s0 = 16.f * scale_of<BF16>(p.x), s1 = 16.f * scale_of<BF16>(p.y), o0 = offset_of<BF16>(p.x) - s0, o1 = offset_of<BF16>(p.y) - s1;
+        const float s0 = scale_of<BF16>(p.x), s1 = scale_of<BF16>(p.y), m0 = offset_of<BF16>(p.x), m1 = offset_of<BF16>(p.y);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          x[u][2 * r + h] = (fmaf(s0, c[0][2 * r + h], s1 * c[1][2 * r + h]) + fmaf(o0, qs[0][h], o1 * qs[1][h])) * factor;
+          x[u][2 * r + h] = fmaf(fmaf(s0, c[0][2 * r + h], s1 * c[1][2 * r + h]), f[h], fmaf(m0, qs[0][h], fmaf(m1, qs[1][h], -ref[h])));
       }
     }
     const auto seen = [&](int u, int e) { return !EDGE || p0 + u * 16 + 8 * (e >> 1) + key_g < sees[e & 1]; };
@@ -328,54 +370,45 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
 #pragma unroll
       for (int r = 0; r < 2; ++r) vp[u][r] = *reinterpret_cast<const uint2*>(st + kOffVP + (u * 16 + 8 * r + key_g) * kParams);
     float top[2] = {fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]))};
-    float far[2] = {1.f, 1.f};                     // what the sums so far are multiplied by
-    bool moves = top[0] > m[0] + kLag || top[1] > m[1] + kLag;
     float s_top = 0.f;
-    if (!BF16) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float s0 = scale_of<BF16>(vp[u][r].x), s1 = scale_of<BF16>(vp[u][r].y);
-          s_top = fmaxf(s_top, fmaxf(s0 < INFINITY ? s0 : 0.f, s1 < INFINITY ? s1 : 0.f));     // (not a NaN either)
-        }
-      moves = moves || s_top > top_scale;
-    }
-    if (__any_sync(0xFFFFFFFFu, moves)) {
+      for (int r = 0; r < 2; ++r) s_top = fmaxf(s_top, fmaxf(scale_of<BF16>(vp[u][r].x), scale_of<BF16>(vp[u][r].y)));      // (fmaxf passes over a NaN)
+    if (__any_sync(0xFFFFFFFFu, top[0] > kLag || top[1] > kLag || m[0] == -INFINITY || m[1] == -INFINITY || s_top > top_scale)) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
         top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], o));
       }
+      float far[2], same = 1.f;                    // what the sums so far are multiplied by
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float n = fmaxf(m[h], top[h]);
+        const float n = fmaxf(m[h], top[h] + ref[h]), r = n == -INFINITY ? 0.f : n;
         far[h] = m[h] == n ? 1.f : exp2_fast(m[h] - n);      // 0 ahead of the first tile
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          x[u][h] -= r - ref[h];
+          x[u][2 + h] -= r - ref[h];
+        }
         m[h] = n;
+        ref[h] = r;
         l[h] *= far[h];
         L[0][h] *= far[h];
         L[1][h] *= far[h];
       }
-      float same = 1.f;
-      if (!BF16) {
-        const float s_all = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(s_top)));
-        if (s_all > top_scale) {                   // twice the next power of two
-          const float n = __uint_as_float((__float_as_uint(s_all) & 0x7F800000u) + 0x01000000u);
-          same = top_scale / n;
-          top_scale = n;
-          inv_scale = 1.f / n;
-        }
+      const uint32_t s_all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(s_top));
+      if (__uint_as_float(s_all) > top_scale) {    // to twice the next power of two
+        const float n = __uint_as_float(min((s_all & 0x7F800000u) + 0x01000000u, 0x7E000000u));
+        same = top_scale / n;
+        top_scale = n;
+        inv_scale = 1.f / n;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) O[i][e] *= far[e & 1] * same;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) C[h][e] *= far[e & 1] * same;
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
     uint32_t w[2][2][2];                           // [16 keys][half][rows of 8]: weights as the second operand
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -383,20 +416,20 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
       for (int r = 0; r < 2; ++r) {
         float p[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) { p[h] = exp2_fast(x[u][2 * r + h] - ref[h]); l[h] += p[h]; }
+        for (int h = 0; h < 2; ++h) { p[h] = exp2_fast(x[u][2 * r + h]); l[h] += p[h]; }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t par = half ? vp[u][r].y : vp[u][r].x;
-          const float s = BF16 ? scale_of<BF16>(par) : scale_of<BF16>(par) * inv_scale, o = offset_of<BF16>(par);
+          const float full = scale_of<BF16>(par), s = full * inv_scale, o = fmaf(8.f, full, offset_of<BF16>(par));
           // a key that a column does not see has no part in it, even where its value is not a number
           if (EDGE) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) L[half][h] = seen(u, 2 * r + h) ? fmaf(p[h], o, L[half][h]) : L[half][h];
-            w[u][half][r] = transpose8(pack2<BF16>(seen(u, 2 * r) ? p[0] * s : 0.f, seen(u, 2 * r + 1) ? p[1] * s : 0.f));
+            w[u][half][r] = transpose8(pack2(seen(u, 2 * r) ? p[0] * s : 0.f, seen(u, 2 * r + 1) ? p[1] * s : 0.f));
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) L[half][h] = fmaf(p[h], o, L[half][h]);
-            w[u][half][r] = transpose8(pack2<BF16>(p[0] * s, p[1] * s));
+            w[u][half][r] = transpose8(pack2(p[0] * s, p[1] * s));
           }
         }
       }
@@ -409,13 +442,11 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
       for (int half = 0; half < 2; ++half) {
         const uint32_t a_ = half ? va.y : va.x, b_ = half ? vb.y : vb.x, c_ = half ? vc.y : vc.x, d_ = half ? vd.y : vd.x;
         // dimensions of the word's low and high 16 bits, of two keys each
-        const uint32_t lo0 = __byte_perm(a_, b_, 0x5410), hi0 = __byte_perm(a_, b_, 0x7632), lo1 = __byte_perm(c_, d_, 0x5410), hi1 = __byte_perm(c_, d_, 0x7632);
+        const Lifted lo0 = levels(__byte_perm(a_, b_, 0x5410), magic), hi0 = levels(__byte_perm(a_, b_, 0x7632), magic);
+        const Lifted lo1 = levels(__byte_perm(c_, d_, 0x5410), magic), hi1 = levels(__byte_perm(c_, d_, 0x7632), magic);
         const uint32_t b0 = w[u][half][0], b1 = w[u][half][1];
-        mma<BF16>(O[4 * half], lift<BF16, 0>(lo0), lift<BF16, 0>(hi0), lift<BF16, 0>(lo1), lift<BF16, 0>(hi1), b0, b1);
-        mma<BF16>(O[4 * half + 1], lift<BF16, 1>(lo0), lift<BF16, 1>(hi0), lift<BF16, 1>(lo1), lift<BF16, 1>(hi1), b0, b1);
-        mma<BF16>(O[4 * half + 2], lift<BF16, 2>(lo0), lift<BF16, 2>(hi0), lift<BF16, 2>(lo1), lift<BF16, 2>(hi1), b0, b1);
-        mma<BF16>(O[4 * half + 3], lift<BF16, 3>(lo0), lift<BF16, 3>(hi0), lift<BF16, 3>(lo1), lift<BF16, 3>(hi1), b0, b1);
-        mma<BF16>(C[half], kOnes, kOnes, kOnes, kOnes, b0, b1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma(O[4 * half + i], lo0.v[i], hi0.v[i], lo1.v[i], hi1.v[i], b0, b1);
       }
     }
   };
@@ -450,13 +481,12 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
     }
   }
   float* po = reinterpret_cast<float*>(ring);      // [column][kOS]
-  const float unit_scale = BF16 ? 16.f : 16.f * top_scale;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int half = i >> 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float2 v = make_float2(fmaf(O[i][h] - C[half][h], unit_scale, L[half][h]), fmaf(O[i][2 + h] - C[half][h], unit_scale, L[half][h]));
+      const float2 v = make_float2(fmaf(O[i][h], top_scale, L[half][h]), fmaf(O[i][2 + h], top_scale, L[half][h]));
       *reinterpret_cast<float2*>(po + (2 * t4 + h) * kOS + 64 * half + 8 * g + 2 * (i & 3)) = v;
     }
   }
