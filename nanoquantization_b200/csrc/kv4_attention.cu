@@ -44,7 +44,7 @@ struct Args {
   const float* cos_sin; int64_t max_positions;
   const int64_t *positions, *rows;
   Cache cache;
-  const int32_t* table; int width;
+  const int32_t* table; int width, shift;         // shift: log2 of the block size, or -1
   const int32_t *ctx;                             // decode
   const int32_t *cu, *pos0;                       // several tokens per sequence
   uint16_t* out;
@@ -73,6 +73,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_from(float (&d)[4], const float (&c)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -189,46 +193,77 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   const int32_t* table = a.table + (int64_t)b * a.width;
 
   // 16-byte piece c of row r at r * 64 + (c ^ 2 bit 2 of r) * 16: eight lanes' pieces lie in different banks for keys (two rows that differ
-  // in their last bit) and for values (four rows, two of each parity, of which two have bit 2 set)
+  // in their last bit) and for values (four rows, two of each parity, of which two have bit 2 set).  A copy takes eight rows at a time.
+  const int l16 = lane & 15;
+  const uint32_t dst_data = ring_a + (lane >> 2) * kData + (((lane & 3) ^ ((lane >> 3) & 2)) << 4), dst_par = ring_a + (lane < 16 ? kOffKP : kOffVP) + l16 * 16;
+  const uint8_t* const par_of = (lane < 16 ? a.cache.k : a.cache.v) + (int64_t)a.cache.block * kData;
+  const auto page_of = [&](int key, int& row) {
+    const int at = a.shift >= 0 ? key >> a.shift : (int)((unsigned)key / (unsigned)a.cache.block);
+    row = key - at * a.cache.block;
+    return table[at];
+  };
   auto load = [&](int t, int stage) {
     if (t < t1) {
       const int p0 = t * kTile;
-      int64_t base[2];
-      int row0[2];
-      bool there[2];
+      const uint32_t dst = dst_data + stage * kStage, par = dst_par + stage * kStage;
+      int row0;
+      const int page = page_of(p0, row0);
+      const bool whole = p0 + kTile <= stored && (unsigned)page < (unsigned)a.cache.pages;
+      // a whole tile of one page, a whole tile of two pages (16 rows lie in one), and any other: 64 sequences of 4000 keys of 8 heads, us,
+      // by the first way, the second and the third: pages of 256 tokens 75, 80, 90; of 16 tokens -, 83, 94
+      int row1 = 0, page1 = -1;
+      if (whole && a.cache.block % kTile != 0) page1 = page_of(p0 + 16, row1);
+      if (whole && a.cache.block % kTile == 0) {
+        const int64_t base = page_at(a.cache, page, kvh);
+        const uint8_t *k = a.cache.k + base + row0 * kData + lane * 16, *v = a.cache.v + base + row0 * kData + lane * 16;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {                // 16 rows lie in one page
-        if (h == 1 && a.cache.block % kTile == 0) { base[1] = base[0]; row0[1] = row0[0] + 16; there[1] = there[0] && p0 + 16 < stored; continue; }
-        const int key = p0 + 16 * h, at = (unsigned)key / (unsigned)a.cache.block;
-        there[h] = key < stored;
-        const int page = there[h] ? table[at] : 0;
-        if (page < 0 || page >= a.cache.pages) { there[h] = false; if (lane == 0) report(a.status, NQB200_ERR_BAD_INDEX); }
-        base[h] = there[h] ? page_at(a.cache, page, kvh) : 0;
-        row0[h] = key - at * a.cache.block;
-      }
-      const uint32_t dst = ring_a + stage * kStage;
-      const int c = lane & 3;
+        for (int i = 0; i < 4; ++i) {
+          copy16(dst + i * 8 * kData, k + i * 8 * kData, 16);
+          copy16(dst + i * 8 * kData + kOffV, v + i * 8 * kData, 16);
+        }
+        copy16(par, par_of + base + (row0 + 2 * l16) * kParams, 16);
+      } else if ((unsigned)page1 < (unsigned)a.cache.pages) {
+        const int64_t base0 = page_at(a.cache, page, kvh), base1 = page_at(a.cache, page1, kvh);
+        const int64_t at0 = base0 + row0 * kData + lane * 16, at1 = base1 + row1 * kData + lane * 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = i >> 1, r = i * 8 + (lane >> 2);
-        const int bytes = there[h] && p0 + r < stored ? 16 : 0;
-        const int64_t src = base[h] + (row0[h] + (r & 15)) * kData + c * 16;
-        const uint32_t to = dst + r * kData + ((c ^ ((r >> 1) & 2)) << 4);
-        copy16(to, a.cache.k + (bytes ? src : 0), bytes);
-        copy16(to + kOffV, a.cache.v + (bytes ? src : 0), bytes);
+        for (int i = 0; i < 4; ++i) {
+          const int64_t at = (i < 2 ? at0 : at1) + (i & 1) * 8 * kData;
+          copy16(dst + i * 8 * kData, a.cache.k + at, 16);
+          copy16(dst + i * 8 * kData + kOffV, a.cache.v + at, 16);
+        }
+        copy16(par, par_of + (l16 < 8 ? base0 : base1) + ((l16 < 8 ? row0 : row1) + 2 * (l16 & 7)) * kParams, 16);
+      } else {
+        int64_t base[2];
+        int row[2];
+        bool there[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = p0 + 16 * h;
+          there[h] = key < stored;
+          const int pg = there[h] ? page_of(key, row[h]) : 0;
+          if (pg < 0 || pg >= a.cache.pages) { there[h] = false; if (lane == 0) report(a.status, NQB200_ERR_BAD_INDEX); }
+          base[h] = there[h] ? page_at(a.cache, pg, kvh) : 0;
+          if (!there[h]) row[h] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int h = i >> 1, r = i * 8 + (lane >> 2), bytes = there[h] && p0 + r < stored ? 16 : 0;
+          const int64_t src = bytes ? base[h] + (row[h] + (r & 15)) * kData + (lane & 3) * 16 : 0;
+          copy16(dst + i * 8 * kData, a.cache.k + src, bytes);
+          copy16(dst + i * 8 * kData + kOffV, a.cache.v + src, bytes);
+        }
+        // parameters of rows 2 l16 and 2 l16 + 1
+        const int left = (l16 < 8 ? there[0] : there[1]) ? stored - (p0 + 2 * l16) : 0, bytes = left >= 2 ? 16 : left == 1 ? 8 : 0;
+        copy16(par, par_of + (bytes ? (l16 < 8 ? base[0] : base[1]) + ((l16 < 8 ? row[0] : row[1]) + 2 * (l16 & 7)) * kParams : 0), bytes);
       }
-      const int l = lane & 15;                     // parameters of rows 2 l and 2 l + 1, of keys and of values
-      const int left = (l < 8 ? there[0] : there[1]) ? stored - (p0 + 2 * l) : 0, bytes = left >= 2 ? 16 : left == 1 ? 8 : 0;
-      const int64_t src = bytes ? (l < 8 ? base[0] : base[1]) + (int64_t)a.cache.block * kData + ((l < 8 ? row0[0] : row0[1]) + 2 * (l & 7)) * kParams : 0;
-      copy16(dst + (lane < 16 ? kOffKP : kOffVP) + l * 16, (lane < 16 ? a.cache.k : a.cache.v) + src, bytes);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) load(t0 + warp + s * kWarps, s);
 
   // queries into fx.q: half a warp each
-  const int unit = tid >> 4, l16 = tid & 15;
+  const int unit = tid >> 4;
   if (DECODE) {
     if (keys > 0) {
       int64_t pos = a.positions[b];
@@ -341,11 +376,12 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
     for (int u = 0; u < 2; ++u) {                  // 16 keys
       const uint4 ka = *reinterpret_cast<const uint4*>(st + u * 16 * kData + koff), kb = *reinterpret_cast<const uint4*>(st + (u * 16 + 8) * kData + koff);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-      float c[2][4] = {{start[0][0], start[0][1], start[0][0], start[0][1]}, {start[1][0], start[1][1], start[1][0], start[1][1]}};
+      float c[2][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const Lifted la = lift(wa[j], magic), lb = lift(wb[j], magic);
-        mma(c[j & 1], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
+        if (j < 2) mma_from(c[j], start[j], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
+        else mma(c[j & 1], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
         mma(c[j & 1], la.v[2], lb.v[2], la.v[3], lb.v[3], qf[j][2], qf[j][3]);
       }
 #pragma unroll
@@ -605,6 +641,7 @@ template <bool BF16, bool DECODE, int STAGES> int launch_stages(const Args& a, i
 template <bool BF16, bool DECODE> int launch_t(Args& a, int64_t batch, int64_t tokens, int64_t keys, cudaStream_t st) {
   const Split s = split((int64_t)a.cache.kv_heads * a.groups * batch, keys);
   a.parts = s.parts;
+  a.shift = (a.cache.block & (a.cache.block - 1)) == 0 ? __builtin_ctz((unsigned)a.cache.block) : -1;
   const int rc = s.stages == 4 ? launch_stages<BF16, DECODE, 4>(a, s.csize, batch, st) : launch_stages<BF16, DECODE, 2>(a, s.csize, batch, st);
   if (rc != NQB200_OK || s.parts == 1) return rc;
   return launch_overlapped(kv4_shares_kernel<BF16>, dim3((unsigned)(tokens * a.heads)), dim3(kDim), 0, st, (const float*)a.shares, a.out, s.parts);
