@@ -23,7 +23,7 @@
 // shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
 #include <cooperative_groups.h>
 #include <type_traits>
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 
 namespace nqb200 {
 namespace {
@@ -35,7 +35,6 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32, kCols = 8;
 constexpr int kStage = kTile * 2 * kToken;                    // keys, values, parameters of keys, parameters of values
 constexpr int kOffV = kTile * kData, kOffKP = 2 * kTile * kData, kOffVP = kOffKP + kTile * kParams;
 constexpr int kOS = kDim + 4;                                 // floats of a column's partial sums
-constexpr int kShare = kDim + 4;                              // floats of a column's share: sums, maximum, sum of weights
 constexpr float kLog2e = 1.4426950408889634f, kLag = 8.f;
 
 struct Args {
@@ -601,6 +600,14 @@ __global__ void __launch_bounds__(kDim) kv4_shares_kernel(const float* __restric
   out[row * kDim + threadIdx.x] = float_to_raw16<BF16>(sum == 0.f ? 0.f : o / sum);
 }
 
+}  // namespace
+
+int kv4::add_shares(const float* shares, uint16_t* out, int64_t rows, int parts, bool bf16, cudaStream_t st) {
+  return launch_overlapped(bf16 ? kv4_shares_kernel<true> : kv4_shares_kernel<false>, dim3((unsigned)rows), dim3(kDim), 0, st, shares, out, parts);
+}
+
+namespace {
+
 // How a call is split: CTAs of a cluster, clusters of a sequence, tiles of a warp's ring.
 constexpr int kResident[4][2] = {{296, 592}, {148, 296}, {71, 142}, {33, 66}};   // clusters of 1, 2, 4, 8 CTAs that are resident with rings of 4 and 2 tiles
 constexpr int kMostParts = 16;
@@ -644,7 +651,7 @@ template <bool BF16, bool DECODE> int launch_t(Args& a, int64_t batch, int64_t t
   a.shift = (a.cache.block & (a.cache.block - 1)) == 0 ? __builtin_ctz((unsigned)a.cache.block) : -1;
   const int rc = s.stages == 4 ? launch_stages<BF16, DECODE, 4>(a, s.csize, batch, st) : launch_stages<BF16, DECODE, 2>(a, s.csize, batch, st);
   if (rc != NQB200_OK || s.parts == 1) return rc;
-  return launch_overlapped(kv4_shares_kernel<BF16>, dim3((unsigned)(tokens * a.heads)), dim3(kDim), 0, st, (const float*)a.shares, a.out, s.parts);
+  return add_shares(a.shares, a.out, tokens * a.heads, s.parts, BF16, st);
 }
 template <bool DECODE> int launch(Args& a, int64_t batch, int64_t tokens, int64_t keys, int dtype, cudaStream_t st) {
   return dtype == NQB200_BF16 ? launch_t<true, DECODE>(a, batch, tokens, keys, st) : launch_t<false, DECODE>(a, batch, tokens, keys, st);
@@ -698,6 +705,8 @@ extern "C" int nqb200_kv4_decode_attention(const void* qkv, int64_t row_stride, 
 
 extern "C" size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads, int64_t kv_heads) {
   if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || batch > 65535 || T <= 0 || max_len <= 0 || max_ctx < max_len) return 0;
+  if (kv4::prompt_umma_supports(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads))
+    return kv4::prompt_umma_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads);
   return scratch_bytes_of(batch, T, max_len, max_ctx, num_q_heads, kv_heads);
 }
 
@@ -711,12 +720,16 @@ extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, cons
     return NQB200_ERR_BAD_SHAPE;
   if (batch == 0 || T == 0) return NQB200_OK;
   const int64_t groups = groups_of(max_len, num_q_heads, cache->kv_heads);
-  if (max_len == 0 || cache->kv_heads * groups > 65535) return NQB200_ERR_BAD_SHAPE;
+  const bool umma = kv4::prompt_umma_supports(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);
+  if (max_len == 0 || (!umma && cache->kv_heads * groups > 65535)) return NQB200_ERR_BAD_SHAPE;
   if (!q || !table || !cu || !pos0 || !out) return NQB200_ERR_NULL_POINTER;
   if (!aligned16(q) || !aligned16(out)) return NQB200_ERR_MISALIGNED;
   const size_t need = nqb200_kv4_prompt_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);
   if (need > 0 && (!scratch || scratch_bytes < need)) return NQB200_ERR_WORKSPACE;
   if (need > 0 && !aligned16(scratch)) return NQB200_ERR_MISALIGNED;
+  if (umma)
+    return kv4::prompt_umma((const uint16_t*)q, q_stride, cache, table, table_width, cu, pos0, (uint16_t*)out, batch, T, max_len, max_ctx, tiles, num_q_heads, scale, dtype,
+                            scratch, status, (cudaStream_t)stream);
   Args a = {};
   a.q = (const uint16_t*)q; a.stride = q_stride; a.cache = kv4::cache_of(cache); a.table = table; a.width = (int)table_width; a.cu = cu; a.pos0 = pos0;
   a.out = (uint16_t*)out; a.heads = (int)num_q_heads; a.groups = (int)groups; a.tokens = (int)T; a.max_len = (int)max_len; a.scale = scale; a.status = status; a.shares = (float*)scratch;
