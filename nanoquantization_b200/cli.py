@@ -8,7 +8,8 @@ spaces or commas); the continuation's ids are printed, one line per prompt.
     {"step": 0, "entries": [{"id": "a", "tokens": [5, 17, 3], "want": [0, 2]}], "end": []}
 
 ``entries`` brings the next tokens of some requests and the places among them whose logits are wanted, ``end`` names
-the requests that are finished after the step.  The wanted logits go to ``OUT/<step>.f32`` (little-endian floats,
+the requests that are finished after the step.  A request's first entry may name another with ``"from"``: it goes on from where that one stood
+before the step, and the two share what the cache holds of it.  The wanted logits go to ``OUT/<step>.f32`` (little-endian floats,
 [wanted, vocab], in the order of the entries), and ``done <step>`` is printed after every step.
 
 Both compile the kernel libraries the model needs if they are missing or out of date."""
@@ -50,7 +51,7 @@ def _generate(args) -> int:
     prompts = [[int(t) for t in line.replace(",", " ").split()] for line in sys.stdin if line.strip()]
     longest = max((len(p) for p in prompts), default=0) + args.max_new_tokens + 1
     blocks = args.blocks or min(args.max_batch, max(len(prompts), 1)) * -(-longest // args.block_size)
-    engine = LLMEngine(model, num_blocks=blocks, block_size=args.block_size, max_batch=args.max_batch, prefill_portion=args.portion)
+    engine = LLMEngine(model, num_blocks=blocks, block_size=args.block_size, max_batch=args.max_batch, prefill_portion=args.portion, kv_bits=args.kv_bits)
     for out in engine.generate(prompts, args.max_new_tokens):
         print(" ".join(map(str, out)), flush=True)
     return 0
@@ -61,15 +62,20 @@ def _trace(args) -> int:
     if model is None:
         return code
     import torch
+    from .csrc import build
     from .engine import LLMEngine, Sequence
     blocks = -(-args.max_tokens // TRACE_BLOCK) + TRACE_REQUESTS
-    engine = LLMEngine(model, num_blocks=blocks, block_size=TRACE_BLOCK, max_batch=TRACE_REQUESTS)
+    engine = LLMEngine(model, num_blocks=blocks, block_size=TRACE_BLOCK, max_batch=TRACE_REQUESTS, kv_bits=args.kv_bits)
     live: dict[str, Sequence] = {}
     for line in sys.stdin:
         if not line.strip():
             continue
         step = json.loads(line)
         entries = []
+        for e in step["entries"]:      # ahead of the step's tokens
+            if e["id"] not in live and e.get("from") is not None:
+                build.build_library(build.LIB_PATH)      # of the copies
+                live[e["id"]] = engine.fork(live[e["from"]])
         for e in step["entries"]:
             seq = live.get(e["id"])
             if seq is None:
@@ -95,6 +101,7 @@ def main(argv=None) -> int:
     for p in (g, t):
         p.add_argument("--model", required=True, help="folder with config.json and *.safetensors")
         p.add_argument("--dtype", default="bfloat16", choices=DTYPES)
+        p.add_argument("--kv-bits", type=int, default=16, choices=(4, 16), help="bits of the cached keys and values (4: Qwen3 with heads of 128)")
     g.add_argument("--max-new-tokens", type=int, default=16)
     g.add_argument("--max-batch", type=int, default=64)
     g.add_argument("--block-size", type=int, default=256)

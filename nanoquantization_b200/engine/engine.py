@@ -10,7 +10,8 @@ paged-KV kernel when that library loads on this GPU, else scaled_dot_product_att
 each sequence.  Qwen3 with heads of 128 has a kernel of its own for decode steps and does not ask for it there.  Other models
 bring kernels that read the cache and the states themselves.
 
-Layout: per layer run two tensors ``[num_blocks, block_size, kv_heads, head_dim]``; a sequence owns a list of blocks;
+Layout: per layer run two tensors ``[num_blocks, block_size, kv_heads, head_dim]``, or with a cache of 4 bits two byte tensors
+(layers/kv4.py); a sequence owns a list of blocks, which forks of it share until one writes;
 ``row = block * block_size + offset``.  Blocks that no later query can reach (every layer attends inside chunks) are
 given back while the sequence runs.  A recurrent state is a row of ``[slots, ...]``; a sequence owns one slot.
 """
@@ -24,6 +25,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from ..layers import kv4
+from ..layers.pages import copy_pages
 from .batch import CacheLayout, StepBatch, to_device
 
 
@@ -49,11 +52,15 @@ class Sequence:
 
 
 class BlockManager:
-    """Free-list allocator of KV-cache blocks."""
+    """Free-list allocator of KV-cache blocks.  A block may be held by several sequences (``share``); before one of them writes into
+    it, ``ensure`` gives that one a block of its own.  What such blocks held is copied by ``flush``, which whoever runs a step calls first."""
 
     def __init__(self, num_blocks: int, block_size: int):
         self.block_size = block_size
         self.free = deque(range(num_blocks))
+        self.shared: dict[int, int] = {}            # block -> holders beyond the first
+        self.copies: list[tuple[int, int]] = []     # (from, to) that a flush still has to copy
+        self.copy = None                            # called with such a list
 
     def blocks_needed(self, n_tokens: int) -> int:
         return -(-n_tokens // self.block_size)
@@ -62,36 +69,71 @@ class BlockManager:
         return self.blocks_needed(n_tokens) <= len(self.free)
 
     def ensure(self, seq: Sequence, n_tokens: int) -> bool:
-        """Grow ``seq`` to hold ``n_tokens``; False (and no change) if the pool is exhausted."""
+        """Grow ``seq`` to hold ``n_tokens``, all blocks from ``seq.computed`` on its own; False (and no change) if the pool is exhausted."""
         need = self.blocks_needed(n_tokens) - len(seq.blocks)
-        if need > len(self.free):
+        others = [i for i in range(seq.computed // self.block_size, len(seq.blocks)) if seq.blocks[i] in self.shared] if self.shared else []
+        if max(need, 0) + len(others) > len(self.free):
             return False
+        for i in others:
+            old, seq.blocks[i] = seq.blocks[i], self.free.popleft()
+            if i * self.block_size < seq.computed:      # it holds tokens that came before
+                self.copies.append((old, seq.blocks[i]))
+            self._let_go(old)
         for _ in range(max(need, 0)):
             seq.blocks.append(self.free.popleft())
         return True
+
+    def share(self, seq: Sequence, other: Sequence) -> None:
+        """``other`` holds what ``seq`` holds."""
+        self.flush()
+        for b in seq.blocks:
+            if b >= 0:
+                self.shared[b] = self.shared.get(b, 0) + 1
+        other.blocks = list(seq.blocks)
+
+    def flush(self) -> None:
+        if self.copies:
+            pairs, self.copies = self.copies, []
+            self.copy(pairs)
+
+    def _let_go(self, block: int) -> None:
+        holders = self.shared.pop(block, 0)
+        if holders > 1:
+            self.shared[block] = holders - 1
+        elif holders == 0:
+            self.free.append(block)
 
     def reclaim(self, seq: Sequence, first_visible: int) -> None:
         """Give back the blocks that lie wholly before ``first_visible`` (their places in the list become -1)."""
         i = min(first_visible // self.block_size, len(seq.blocks)) - 1
         while i >= 0 and seq.blocks[i] >= 0:
-            self.free.append(seq.blocks[i])
+            self.flush()
+            self._let_go(seq.blocks[i])
             seq.blocks[i] = -1
             i -= 1
 
     def release(self, seq: Sequence) -> None:
-        self.free.extend(b for b in seq.blocks if b >= 0)
+        self.flush()        # a block that goes back to the pool is no part of a copy
+        for b in seq.blocks:
+            if b >= 0:
+                self._let_go(b)
         seq.blocks = []
 
 
 class PagedKVCache:
-    """Keys and values of every layer run that keeps some (None for the others)."""
+    """Keys and values of every layer run that keeps some (None for the others): ``[num_blocks, block_size, kv_heads, head_dim]`` of
+    ``dtype``, or with ``bits`` = 4 the byte tensors of ``layers/kv4.py``."""
 
-    def __init__(self, layout: CacheLayout, num_blocks, block_size, dtype, device):
+    def __init__(self, layout: CacheLayout, num_blocks, block_size, dtype, device, bits: int = 16):
         def pool(heads, dim):
             return torch.zeros(num_blocks, block_size, heads, dim, dtype=dtype, device=device)
-        self.k = [None if s is None else pool(s.kv_heads, s.head_dim) for s in layout.kv]
-        self.v = [None if s is None else pool(s.kv_heads, s.v_dim) for s in layout.kv]
-        self.block_size = block_size
+        if bits == 4:
+            pairs = [(None, None) if s is None else kv4.new_cache(num_blocks, block_size, s.kv_heads, device) for s in layout.kv]
+            self.k, self.v = [k for k, _ in pairs], [v for _, v in pairs]
+        else:
+            self.k = [None if s is None else pool(s.kv_heads, s.head_dim) for s in layout.kv]
+            self.v = [None if s is None else pool(s.kv_heads, s.v_dim) for s in layout.kv]
+        self.block_size, self.bits = block_size, bits
 
     def write(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         self.k[layer].view(-1, *k.shape[1:]).index_copy_(0, slots, k)
@@ -127,6 +169,8 @@ class LayerStep:
     def __init__(self, engine: "LLMEngine", run: int, batch: StepBatch, decode: bool):
         self.engine, self.batch, self.decode = engine, batch, decode
         self.k_cache, self.v_cache, self.state = engine.cache.k[run], engine.cache.v[run], engine.states.states[run]
+        # a cache of 4 bits is written and read by its own kernels (layers/kv4.py), which the model calls
+        self.kv4 = (self.k_cache, self.v_cache, batch) if engine.cache.bits == 4 else None
         self.kv_target = (self.k_cache, self.v_cache, batch.rows)
         # what a kernel that looks up the pages itself needs for a decode step (heads of 128; other sizes call this object)
         self.paged_decode = (self.k_cache, self.v_cache, batch) if decode and self.k_cache is not None and self.k_cache.is_cuda else None
@@ -263,19 +307,30 @@ class Scheduler:
 
 class LLMEngine:
     def __init__(self, model, num_blocks: int, block_size: int = 256, max_batch: int = 64,
-                 max_prefill_tokens: int = 16384, use_cuda_graph: bool = True, prefill_portion: Optional[int] = None):
+                 max_prefill_tokens: int = 16384, use_cuda_graph: bool = True, prefill_portion: Optional[int] = None, kv_bits: int = 16):
+        """``kv_bits``: 16 keeps keys and values in the model's type, 4 quantises them (3.6 times as many tokens in the same memory;
+        for models that leave attention to the engine, in a 16-bit type, with heads of 128)."""
         self.model = model
         self.device, self.dtype = model.device, model.dtype
         self.layout = model.cache_layout()
         self.block_size = block_size
+        if kv_bits not in (4, 16):
+            raise ValueError(f"keys and values are kept in 4 or 16 bits, not {kv_bits}")
+        if kv_bits == 4:
+            if not model.delegates_attention or self.dtype not in (torch.float16, torch.bfloat16) or any(
+                    s is None or s.head_dim != kv4.DIM or s.v_dim != kv4.DIM or s.chunk for s in self.layout.kv):
+                raise ValueError(f"a 4-bit cache is for models that leave attention to the engine, in float16 or bfloat16, with heads of {kv4.DIM}")
+            if block_size % 16:
+                raise ValueError(f"a 4-bit cache takes blocks of a multiple of 16 tokens, got {block_size}")
         # one block and one slot more than are handed out: padding rows of a bucketed decode batch write there
-        self.cache = PagedKVCache(self.layout, num_blocks + 1, block_size, self.dtype, self.device)
+        self.cache = PagedKVCache(self.layout, num_blocks + 1, block_size, self.dtype, self.device, kv_bits)
         self.states = StatePool(self.layout, max_batch + 1, self.device)
         self.scratch_block, self.scratch_slot = num_blocks, max_batch
         self.blocks = BlockManager(num_blocks, block_size)
+        self.blocks.copy = self._copy_blocks
         self.scheduler = Scheduler(self.blocks, max_batch, max_prefill_tokens, prefill_portion, self.states)
         self.use_cuda_graph = use_cuda_graph
-        self.paged_attention = self._probe_flash_attn() if model.delegates_attention and block_size % 256 == 0 else None
+        self.paged_attention = self._probe_flash_attn() if model.delegates_attention and block_size % 256 == 0 and kv_bits == 16 else None
         self._graphs: dict[tuple[int, int], tuple] = {}
         self._warm_stream = None  # one side stream for every graph warm-up (scratch buffers are kept per stream)
         self._next_id = 0
@@ -298,6 +353,16 @@ class LLMEngine:
             return None
 
     # --------------------------------------------------------------------- steps
+    def _copy_rows(self, pools: list[torch.Tensor], pairs: list[tuple[int, int]]) -> None:
+        if self.device.type == "cuda":
+            copy_pages(pools, [a for a, _ in pairs], [b for _, b in pairs])
+        else:
+            for p in pools:
+                p[[b for _, b in pairs]] = p[[a for a, _ in pairs]]
+
+    def _copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
+        self._copy_rows([p for p in self.cache.k + self.cache.v if p is not None], pairs)
+
     def _forward(self, batch: StepBatch, decode: bool, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         return self.model.forward_step(batch, lambda run: LayerStep(self, run, batch, decode), rows)
 
@@ -320,6 +385,7 @@ class LLMEngine:
                               [self.scratch_slot if s.slot is None else s.slot for s in batch], width, self.block_size)
         if rows is None:
             rows = host.cu.numpy()[1:] - 1
+        self.blocks.flush()
         rows = rows.astype(np.int64)
         everything = np.array_equal(rows, np.arange(host.num_tokens))
         h = self._forward(host.to(self.device), False, None if everything else to_device(torch.from_numpy(rows), self.device))
@@ -355,6 +421,7 @@ class LLMEngine:
         """One token of every sequence: final hidden states and greedy choices."""
         B = len(batch)
         width = max(1, max(len(s.blocks) for s in batch))
+        self.blocks.flush()
         if not self.use_cuda_graph:
             h, out = self._decode_forward(self._decode_inputs(batch, width).to(self.device))
         else:
@@ -363,7 +430,7 @@ class LLMEngine:
             # table keeps its exact width, by which flash_attn sizes its KV splits (a table padded from 9 to 16 blocks cost
             # 18 % of a step); kernels that look up their own pages take a width rounded up as well
             rows = 1 << (B - 1).bit_length()
-            if not self.model.delegates_attention:
+            if not self.model.delegates_attention or self.cache.bits == 4:
                 width = 1 << (width - 1).bit_length()
             host = self._decode_inputs(batch, width, rows)
             key = (rows, width)
@@ -421,6 +488,18 @@ class LLMEngine:
             o += len(want)
         return out
 
+    def fork(self, s: Sequence) -> Sequence:
+        """A sequence that goes on, with ``extend``, from where ``s`` stands, which goes on as well.  They share the blocks of what they have in
+        common; one that writes into a shared block gets a copy of it first.  Recurrent states are copied at once."""
+        t = Sequence(s.seq_id, list(s.prompt), s.max_new_tokens, list(s.output))
+        t.prefilled, t.carried, t.computed = s.prefilled, list(s.carried), s.computed
+        if self.layout.recurrent and s.slot is not None:
+            if not self.states.ensure(t):
+                raise RuntimeError(f"no state slot is free for a fork of sequence {s.seq_id}")
+            self._copy_rows([p for run in self.states.states for p in run.values()], [(s.slot, t.slot)])
+        self.blocks.share(s, t)
+        return t
+
     def drop(self, s: Sequence) -> None:
         """Give back what a sequence holds."""
         self.scheduler.release(s)
@@ -465,6 +544,7 @@ class LLMEngine:
         if self.device.type == "cuda":
             _lib.check_workspaces()
             _lib.check_mixer_status()
+            _lib.check_cache_status()
 
     def generate(self, prompts: Seq[Seq[int]], max_new_tokens) -> list[list[int]]:
         if isinstance(max_new_tokens, int):

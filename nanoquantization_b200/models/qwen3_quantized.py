@@ -27,7 +27,7 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..layers import fused
+from ..layers import fused, kv4
 from ..layers.gemm import WQLinear_GEMM  # noqa: F401  (the class every projection derives from)
 from ..layers.parallel import ColumnParallelWQLinear, MergedColumnParallelWQLinear, RowParallelWQLinear
 
@@ -168,6 +168,10 @@ class Qwen3QuantizedAttention(nn.Module):
         else:
             qkv = torch.cat([self.q_proj(x), self.k_proj(x), self.v_proj(x)], dim=-1)
         stored = False
+        quantised = getattr(attend, "kv4", None)
+        if quantised is not None:  # a cache of 4 bits: its kernels store and read it
+            o = self._attend_kv4(qkv, positions, *quantised, attend.decode)
+            return self.o_proj.forward_residual(o, residual) if residual is not None else self.o_proj(o)
         paged = getattr(attend, "paged_decode", None) if self.head_dim == 128 else None
         if paged is not None:  # a decode step over a paged cache: norm, rotation, K/V store and attention in one launch
             k_cache, v_cache, batch = paged
@@ -191,6 +195,14 @@ class Qwen3QuantizedAttention(nn.Module):
         if residual is not None:  # (new residual stream, its per-tile sums of squares) from o_proj's own launches
             return self.o_proj.forward_residual(o, residual)
         return self.o_proj(o)
+
+
+    def _attend_kv4(self, qkv, positions, k_cache, v_cache, batch, decode: bool) -> torch.Tensor:
+        args = (qkv, self.q_norm.weight, self.k_norm.weight, self.rope.cos_sin_cache, positions, self.num_heads, self.num_kv_heads, self.q_norm.eps, k_cache, v_cache)
+        if decode:
+            return kv4.decode_attention(*args, batch.table, batch.ctx, batch.rows)
+        q = kv4.qknorm_rope_store(*args, batch.rows)
+        return kv4.prompt_attention(q, self.num_heads, k_cache, v_cache, batch.table, batch.cu, batch.pos0, batch.lens, batch.starts)
 
 
 class Qwen3QuantizedMLP(nn.Module):

@@ -101,3 +101,109 @@ def test_the_layout_reads_back_what_it_packs(dtype):
 
 def test_a_zero_filled_cache_reads_as_zeros():
     assert not ref.unpack(torch.zeros(3, 64, dtype=torch.uint8), torch.zeros(3, 8, dtype=torch.uint8), torch.float16).any()
+
+
+# ------------------------------------------------------------------ blocks that sequences share
+def _manager(blocks=8, size=4):
+    from nanoquantization_b200.engine import BlockManager
+    m, log = BlockManager(blocks, size), []
+    m.copy = lambda pairs: log.append(list(pairs))
+    return m, log
+
+
+def test_a_shared_block_is_copied_before_one_writes_into_it():
+    from nanoquantization_b200.engine import Sequence
+    m, log = _manager()
+    a, b = Sequence(0, [1] * 10, 9), Sequence(1, [1] * 10, 9)
+    assert m.ensure(a, 10)
+    a.computed = b.computed = 10
+    m.share(a, b)
+    assert b.blocks == a.blocks and len(m.free) == 5
+    assert m.ensure(a, 11) and a.blocks[:2] == b.blocks[:2] and a.blocks[2] != b.blocks[2]      # the one with token 10 in it
+    assert m.copies == [(b.blocks[2], a.blocks[2])] and not log
+    assert m.ensure(b, 11) and len(m.copies) == 1                                               # the other has it to itself now
+    m.flush()
+    assert log == [[(b.blocks[2], a.blocks[2])]] and not m.copies
+    m.release(a)
+    assert len(m.free) == 5 and set(m.free).isdisjoint(b.blocks)
+    m.release(b)
+    assert sorted(m.free) == list(range(8)) and not m.shared
+
+
+def test_blocks_that_hold_nothing_yet_are_replaced_and_not_copied():
+    from nanoquantization_b200.engine import Sequence
+    m, log = _manager()
+    a, b = Sequence(0, [1] * 8, 9), Sequence(1, [1] * 8, 9)
+    assert m.ensure(a, 9)                   # a block more than the eight tokens that there are
+    a.computed = b.computed = 8
+    m.share(a, b)
+    assert m.ensure(b, 9) and b.blocks[2] != a.blocks[2] and not m.copies and len(m.free) == 4
+
+
+def test_no_change_where_there_is_no_room_for_a_copy():
+    from nanoquantization_b200.engine import Sequence
+    m, log = _manager(3)
+    a, b = Sequence(0, [1] * 10, 9), Sequence(1, [1] * 10, 9)
+    assert m.ensure(a, 10)
+    a.computed = b.computed = 10
+    m.share(a, b)
+    before = list(b.blocks)
+    assert not m.ensure(b, 11) and b.blocks == before and not m.copies and m.shared == {x: 1 for x in before}
+    m.release(a)
+    assert not m.free and m.ensure(b, 11) and b.blocks == before
+
+
+def test_copies_run_before_their_blocks_change_hands():
+    from nanoquantization_b200.engine import Sequence
+    m, log = _manager()
+    seqs = [Sequence(i, [1] * 6, 9) for i in range(3)]
+    assert m.ensure(seqs[0], 6)
+    for s in seqs:
+        s.computed = 6
+    m.share(seqs[0], seqs[1]), m.share(seqs[0], seqs[2])
+    assert all(m.ensure(s, 7) for s in seqs) and len(m.copies) == 2 and len({s.blocks[1] for s in seqs}) == 3
+    pending = list(m.copies)
+    m.release(seqs[1])                      # its blocks go back to the pool: the copies have run
+    assert log == [pending] and not m.copies
+    t = Sequence(4, [], 1)
+    m.share(seqs[0], t)
+    m.reclaim(seqs[0], 4)
+    assert seqs[0].blocks[0] == -1 and t.blocks[0] >= 0 and t.blocks[0] not in m.free
+    for s in (seqs[0], seqs[2], t):
+        m.release(s)
+    assert sorted(m.free) == list(range(8)) and not m.shared
+
+
+def test_engines_that_a_4_bit_cache_is_not_for():
+    from nanoquantization_b200.engine import LLMEngine
+    from nanoquantization_b200.models.qwen3_quantized import Qwen3QuantizedForCausalLM
+    make = lambda dim, dtype: Qwen3QuantizedForCausalLM(1, 64, 256, 256 // dim, 1, 32, 128, 4, 128, dim, device="cpu", dtype=dtype)  # noqa: E731
+    with pytest.raises(ValueError, match="heads of 128"):
+        LLMEngine(make(64, torch.float16), num_blocks=2, block_size=16, kv_bits=4)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        LLMEngine(make(128, torch.float16), num_blocks=2, block_size=8, kv_bits=4)
+    with pytest.raises(ValueError, match="4 or 16 bits"):
+        LLMEngine(make(128, torch.float16), num_blocks=2, block_size=16, kv_bits=8)
+    engine = LLMEngine(make(128, torch.bfloat16), num_blocks=2, block_size=16, max_batch=2, kv_bits=4)
+    assert engine.cache.bits == 4 and engine.cache.k[0].shape == (3, 1, 16 * 72) and engine.cache.k[0].dtype == torch.uint8
+
+
+def test_a_fork_holds_what_its_sequence_holds():
+    from nanoquantization_b200.engine import LLMEngine, Sequence
+    from nanoquantization_b200.models.qwen3_quantized import Qwen3QuantizedForCausalLM
+    model = Qwen3QuantizedForCausalLM(1, 64, 256, 2, 1, 32, 128, 4, 128, 128, device="cpu", dtype=torch.float16)
+    engine = LLMEngine(model, num_blocks=6, block_size=4, max_batch=2, use_cuda_graph=False)
+    s = Sequence(3, [5, 6, 7, 8, 9, 10], 4, [11])
+    assert engine.blocks.ensure(s, 7)
+    s.computed = 6
+    for c in (engine.cache.k[0], engine.cache.v[0]):
+        c.copy_(torch.randn(c.shape))
+    t = engine.fork(s)
+    assert (t.prompt, t.output, t.blocks, t.computed, t.max_new_tokens) == (s.prompt, s.output, s.blocks, 6, 4) and t.prompt is not s.prompt
+    before = engine.cache.k[0].clone()
+    engine._hold(t, 8)
+    assert t.blocks[0] == s.blocks[0] and t.blocks[1] != s.blocks[1]
+    engine.blocks.flush()
+    assert torch.equal(engine.cache.k[0][t.blocks[1]], before[s.blocks[1]])
+    engine.drop(s), engine.drop(t)
+    assert sorted(engine.blocks.free) == list(range(6))
