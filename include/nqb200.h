@@ -231,7 +231,7 @@ typedef struct nqb200_kv4 {
 
 /* Tokens of a prompt step: q_out [T, num_q_heads * 128] takes the queries of qkv [T, row_stride] after head norm and rotation (as
  * nqb200_qknorm_rope, but computed in 32 bits and rounded once), cache row rows[t] takes the keys, normed and rotated, and the values.
- * A row below 0: the token is not stored.  qkv is left as it is.  cos_sin: [max_positions, 128].  row_stride a multiple of 4. */
+ * A row below 0: the token is not stored.  qkv is left as it is.  cos_sin: [max_positions, 128].  row_stride a multiple of 4; 8-byte alignment does for qkv and the weights. */
 int nqb200_kv4_store(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
                      int64_t max_positions, const int64_t* positions, const int64_t* rows, const nqb200_kv4* cache, void* q_out, int64_t T,
                      int64_t num_q_heads, float eps, int dtype, int* status, void* stream);

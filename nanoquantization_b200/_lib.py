@@ -65,7 +65,7 @@ SIGNATURES = {
     "nqb200_kv4_decode_scratch_bytes": (_sz, [_i64] * 5),
     "nqb200_kv4_prompt_attention": (_int, [_vp, _i64, _kv4, _vp, _i64, _vp, _vp, _vp] + [_i64] * 6 + [ctypes.c_float, _int, _vp, _sz, _vp, _vp]),
     "nqb200_kv4_prompt_scratch_bytes": (_sz, [_i64] * 7),
-    "nqb200_copy_pages": (_int, [ctypes.POINTER(_vp), ctypes.POINTER(_i64), _i64, _i64, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), _i64, _vp]),
+    "nqb200_copy_pages": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "nqb200_silu_mul": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "nqb200_comm_alloc": (_int, [ctypes.POINTER(_vp), _sz]),
     "nqb200_comm_free": (_int, [_vp]),
@@ -250,18 +250,17 @@ def check_mixer_status() -> None:
 
 
 class on_device:
-    """Makes a tensor's device the current one for a call; gives the device's index and its current stream."""
-    __slots__ = ("index", "before", "stream")
+    """Makes a GPU the current one for a call, and gives its current stream."""
+    __slots__ = ("index", "before")
 
-    def __init__(self, dev: torch.device):
-        self.before = torch.cuda.current_device()
-        self.index = self.before if dev.index is None else dev.index
+    def __init__(self, index: int):
+        self.index = index
 
-    def __enter__(self):
+    def __enter__(self) -> int:
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        self.stream = stream_of(self.index)
-        return self
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:

@@ -110,49 +110,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// A query as the first product's second operand, in units of a power of two that puts its largest element between 256 and 512: half a
-// warp, as for turned(); elements that meet 1024 + 16 n are divided by 16.  Returns the unit.
-__device__ __forceinline__ float operand(const float (&x)[4], const float (&y)[4], uint2& lo, uint2& hi) {
+// A query as the first product's second operand, in units of a power of two that puts its largest element between 256 and 512: eight
+// lanes, as for head_values(); elements that meet 1024 + 16 n are divided by 16.  Returns the unit.
+__device__ __forceinline__ float operand(const float (&x)[8], const float (&y)[8], uint4& lo, uint4& hi) {
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const uint32_t e = min(max(__float_as_uint(top) >> 23, 9u), 253u);
   const float f = __uint_as_float((262u - e) << 23), f16 = f * 0.0625f;
-  lo = make_uint2(pack2(x[0] * f, x[1] * f), pack2(x[2] * f16, x[3] * f16));       // dimensions 4 l .. 4 l + 3: lifted pairs of even and odd number
-  hi = make_uint2(pack2(y[0] * f, y[1] * f), pack2(y[2] * f16, y[3] * f16));
+  lo = make_uint4(pack2(x[0] * f, x[1] * f), pack2(x[2] * f16, x[3] * f16), pack2(x[4] * f, x[5] * f), pack2(x[6] * f16, x[7] * f16));
+  hi = make_uint4(pack2(y[0] * f, y[1] * f), pack2(y[2] * f16, y[3] * f16), pack2(y[4] * f, y[5] * f), pack2(y[6] * f16, y[7] * f16));
   return __uint_as_float((e - 8u) << 23);
-}
-
-// A head after norm and rotation: half a warp, lane l has dimensions 4 l .. and 64 + 4 l ..; `weight` null: as it is.
-template <bool BF16>
-__device__ __forceinline__ void turned(const uint16_t* src, const uint16_t* weight, const float* angles, float eps, float (&x)[4], float (&y)[4]) {
-  const int l = threadIdx.x & 15;
-  const uint2 lo = reinterpret_cast<const uint2*>(src)[l], hi = reinterpret_cast<const uint2*>(src)[l + 16];
-  const uint32_t lw[2] = {lo.x, lo.y}, hw[2] = {hi.x, hi.y};
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[e] = raw16_to_float<BF16>((uint16_t)(lw[e >> 1] >> (16 * (e & 1))));
-    y[e] = raw16_to_float<BF16>((uint16_t)(hw[e >> 1] >> (16 * (e & 1))));
-    ss += x[e] * x[e] + y[e] * y[e];
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-  if (!weight) return;
-  const float inv = rsqrtf(ss / (float)kDim + eps);
-  const uint2 wl = reinterpret_cast<const uint2*>(weight)[l], wh = reinterpret_cast<const uint2*>(weight)[l + 16];
-  const uint32_t wlw[2] = {wl.x, wl.y}, whw[2] = {wh.x, wh.y};
-  const float4 cv = reinterpret_cast<const float4*>(angles)[l], sv = reinterpret_cast<const float4*>(angles)[l + 16];
-  const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float u = x[e] * inv * raw16_to_float<BF16>((uint16_t)(wlw[e >> 1] >> (16 * (e & 1))));
-    const float v = y[e] * inv * raw16_to_float<BF16>((uint16_t)(whw[e >> 1] >> (16 * (e & 1))));
-    x[e] = u * c[e] - v * s[e];
-    y[e] = u * s[e] + v * c[e];
-  }
 }
 
 // STAGES: tiles of a warp's ring (see split()).  DECODE: one token per sequence whose own key and value are made here.
@@ -261,55 +231,49 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
 #pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) load(t0 + warp + s * kWarps, s);
 
-  // queries into fx.q: half a warp each
-  const int unit = tid >> 4;
-  if (DECODE) {
-    if (keys > 0) {
+  // queries into fx.q, eight lanes each: the first two warps; the step's own key and value: the third
+  const int unit = tid >> 3, m8 = tid & 7;
+  if (keys > 0 && (warp < 2 || (newest && warp == 2))) {
+    float x[8], y[8];
+    const int c = min(unit, cols - 1), idx = group * kCols + c;      // (columns beyond `cols` repeat the last one and are not used)
+    const bool is_v = unit == 9;
+    if (DECODE) {
       int64_t pos = a.positions[b];
       if (pos < 0 || pos >= a.max_positions) {
         if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
         pos = 0;
       }
-      const float* angles = a.cos_sin + pos * kDim;
-      const uint16_t* row = a.q + (int64_t)b * a.stride;
-      float x[4], y[4];
-      turned<BF16>(row + (int64_t)(kvh * R + group * kCols + min(unit, cols - 1)) * kDim, a.qw, angles, a.eps, x, y);
-      uint2 lo, hi;
-      const float f = operand(x, y, lo, hi);       // (columns beyond `cols` repeat the last one and are not used)
-      reinterpret_cast<uint2*>(fx.q[unit])[l16] = lo;
-      reinterpret_cast<uint2*>(fx.q[unit])[l16 + 16] = hi;
-      if (l16 == 0) fx.unit[unit] = f;
-      if (newest && warp == 0) {                   // the key and the value
-        const bool is_v = unit == 1;
-        turned<BF16>(row + (int64_t)(a.heads + (is_v ? a.cache.kv_heads : 0) + kvh) * kDim, is_v ? nullptr : a.kw, angles, a.eps, x, y);
-        uint32_t word;
-        uint2 params;
-        quantise<BF16>(x, y, word, params);
-        fx.own[is_v][l16] = word;
-        if (l16 == 0) fx.own_params[is_v] = params;
+      const int head = warp < 2 ? kvh * R + idx : a.heads + (is_v ? a.cache.kv_heads : 0) + kvh;
+      head_values<BF16>(a.q + (int64_t)b * a.stride + (int64_t)head * kDim, warp < 2 ? a.qw : is_v ? nullptr : a.kw, a.cos_sin + pos * kDim, a.eps, x, y);
+    } else {
+      head_values<BF16>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim, nullptr, nullptr, 0.f, x, y);
+    }
+    if (warp < 2) {
+      uint4 lo, hi;
+      const float f = operand(x, y, lo, hi);
+      reinterpret_cast<uint4*>(fx.q[unit])[m8] = lo;
+      reinterpret_cast<uint4*>(fx.q[unit])[m8 + 8] = hi;
+      if (m8 == 0) fx.unit[unit] = f;
+    } else {
+      uint2 words, params;
+      quantise<BF16>(x, y, words, params);
+      if (unit < 10) {
+        reinterpret_cast<uint2*>(fx.own[is_v])[m8] = words;
+        if (m8 == 0) fx.own_params[is_v] = params;
         const int64_t at = a.rows[b];
         if (group == 0 && at >= 0) {
           const int64_t page = at / a.cache.block;
           if (page < a.cache.pages) {
             const int r = (int)(at - page * a.cache.block);
             uint8_t* base = (is_v ? a.cache.v : a.cache.k) + page_at(a.cache, page, kvh);
-            reinterpret_cast<uint32_t*>(base + r * kData)[l16] = word;
-            if (l16 == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
-          } else if (l16 == 0) {
+            reinterpret_cast<uint2*>(base + r * kData)[m8] = words;
+            if (m8 == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
+          } else if (m8 == 0) {
             report(a.status, NQB200_ERR_BAD_INDEX);
           }
         }
       }
     }
-  } else {
-    const int idx = group * kCols + min(unit, cols - 1);
-    float x[4], y[4];
-    turned<BF16>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim, nullptr, nullptr, 0.f, x, y);
-    uint2 lo, hi;
-    const float f = operand(x, y, lo, hi);
-    reinterpret_cast<uint2*>(fx.q[unit])[l16] = lo;
-    reinterpret_cast<uint2*>(fx.q[unit])[l16 + 16] = hi;
-    if (l16 == 0) fx.unit[unit] = f;
   }
   __syncthreads();
 

@@ -1,8 +1,7 @@
 // Store and read-back of the 4-bit key/value cache.
 //
 // Both are bound by memory: a token's projections in (256 bytes a head), its queries out and 144 bytes per key/value head stored.
-// Half a warp per (token, head), 16 lanes with 4 + 4 dimensions that are half a head apart: what the rotation pairs lies in one lane, and
-// the two halves are the two groups of a row.
+// Eight lanes per (token, head), every access 16 bytes wide (8 where a row of nibbles is written).
 #include "kv4.cuh"
 
 namespace nqb200 {
@@ -22,72 +21,42 @@ struct StoreArgs {
   int* status;
 };
 
-template <bool BF16>
+template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ StoreArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 15, Hq = a.heads, Hkv = a.cache.kv_heads, per = Hq + 2 * Hkv;
-  const int at = blockIdx.x * 16 + (threadIdx.x >> 4);
-  const bool in = at < a.T * per;                      // no early return: the other half of the warp may be inside
+  const int m = threadIdx.x & 7, Hq = a.heads, Hkv = a.cache.kv_heads, per = Hq + 2 * Hkv;
+  const int at = blockIdx.x * 32 + (threadIdx.x >> 3);
+  const bool in = at < a.T * per;                      // no early return: other heads of the warp may be inside
   const int t = in ? at / per : 0, hd = in ? at - t * per : 0;
   const bool is_v = hd >= Hq + Hkv, is_q = hd < Hq;
-  const uint2* src = reinterpret_cast<const uint2*>(a.qkv + (int64_t)t * a.stride + (int64_t)hd * kDim);
-  const uint2 lo = src[lane], hi = src[lane + 16];
-  float x[4], y[4];
-  const uint32_t lw[2] = {lo.x, lo.y}, hw[2] = {hi.x, hi.y};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[e] = raw16_to_float<BF16>((uint16_t)(lw[e >> 1] >> (16 * (e & 1))));
-    y[e] = raw16_to_float<BF16>((uint16_t)(hw[e >> 1] >> (16 * (e & 1))));
+  int64_t pos = a.positions[t];
+  if (pos < 0 || pos >= a.max_positions) {
+    if (in && hd == 0 && m == 0) report(a.status, NQB200_ERR_BAD_INDEX);
+    pos = 0;
   }
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-  if (!is_v) {
-    const float inv = rsqrtf(ss / (float)kDim + a.eps);
-    int64_t pos = a.positions[t];
-    if (pos < 0 || pos >= a.max_positions) {
-      if (in && lane == 0) report(a.status, NQB200_ERR_BAD_INDEX);
-      pos = 0;
-    }
-    const uint2* w = reinterpret_cast<const uint2*>(is_q ? a.qw : a.kw);
-    const uint2 wl = w[lane], wh = w[lane + 16];
-    const uint32_t wlw[2] = {wl.x, wl.y}, whw[2] = {wh.x, wh.y};
-    const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + pos * kDim);   // [cos(64) | sin(64)]
-    const float4 cv = cs[lane], sv = cs[lane + 16];
-    const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float u = x[e] * inv * raw16_to_float<BF16>((uint16_t)(wlw[e >> 1] >> (16 * (e & 1))));
-      const float v = y[e] * inv * raw16_to_float<BF16>((uint16_t)(whw[e >> 1] >> (16 * (e & 1))));
-      x[e] = u * c[e] - v * s[e];
-      y[e] = u * s[e] + v * c[e];
-    }
-  }
-  // (the quantisation's shuffles take the whole warp: its other half may be a key or a value)
-  if (__any_sync(0xFFFFFFFFu, in && !is_q)) {
-    uint32_t word;
-    uint2 params;
-    quantise<BF16>(x, y, word, params);
+  float x[8], y[8];
+  head_values<BF16, WIDE>(a.qkv + (int64_t)t * a.stride + (int64_t)hd * kDim, is_v ? nullptr : is_q ? a.qw : a.kw, a.cos_sin + pos * kDim, a.eps, x, y);
+  if (__any_sync(0xFFFFFFFFu, in && !is_q)) {          // (a warp's other heads go along)
+    uint2 words, params;
+    quantise<BF16>(x, y, words, params);
     if (in && !is_q) {
-      const int64_t row = a.rows[t], page = row / a.cache.block;
+      const int64_t row = a.rows[t], page = row >= 0 && row <= INT32_MAX ? (int64_t)((uint32_t)row / (uint32_t)a.cache.block) : row / a.cache.block;
       if (row >= 0 && page < a.cache.pages) {
         const int r = (int)(row - page * a.cache.block);
         uint8_t* base = (is_v ? a.cache.v : a.cache.k) + page_at(a.cache, page, is_v ? hd - Hq - Hkv : hd - Hq);
-        reinterpret_cast<uint32_t*>(base + r * kData)[lane] = word;
-        if (lane == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
-      } else if (row >= 0 && lane == 0) {
+        reinterpret_cast<uint2*>(base + r * kData)[m] = words;
+        if (m == 0) *reinterpret_cast<uint2*>(base + (int64_t)a.cache.block * kData + r * kParams) = params;
+      } else if (row >= 0 && m == 0) {
         report(a.status, NQB200_ERR_BAD_INDEX);
       }
     }
   }
   if (in && is_q) {
-    uint2* dst = reinterpret_cast<uint2*>(a.q_out + ((int64_t)t * Hq + hd) * kDim);
+    uint4* dst = reinterpret_cast<uint4*>(a.q_out + ((int64_t)t * Hq + hd) * kDim);
     const auto pack = [](float p, float q) { return (uint32_t)float_to_raw16<BF16>(p) | ((uint32_t)float_to_raw16<BF16>(q) << 16); };
-    dst[lane] = make_uint2(pack(x[0], x[1]), pack(x[2], x[3]));
-    dst[lane + 16] = make_uint2(pack(y[0], y[1]), pack(y[2], y[3]));
+    dst[m] = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
+    dst[m + 8] = make_uint4(pack(y[0], y[1]), pack(y[2], y[3]), pack(y[4], y[5]), pack(y[6], y[7]));
   }
 }
 
@@ -133,14 +102,16 @@ extern "C" int nqb200_kv4_store(const void* qkv, int64_t row_stride, const void*
     return NQB200_ERR_BAD_SHAPE;
   if (dtype != NQB200_F16 && dtype != NQB200_BF16) return NQB200_ERR_BAD_DTYPE;
   if (T == 0) return NQB200_OK;
-  if (T > (INT32_MAX - 16) / (num_q_heads + 2 * cache->kv_heads)) return NQB200_ERR_TOO_LARGE;
+  if (T > (INT32_MAX - 32) / (num_q_heads + 2 * cache->kv_heads)) return NQB200_ERR_TOO_LARGE;
   if (!qkv || !q_weight || !k_weight || !cos_sin || !positions || !rows || !q_out) return NQB200_ERR_NULL_POINTER;
   const auto on8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; };
-  if (!on8(qkv) || !on8(q_weight) || !on8(k_weight) || !on8(q_out) || !aligned16(cos_sin)) return NQB200_ERR_MISALIGNED;
+  if (!on8(qkv) || !on8(q_weight) || !on8(k_weight) || !aligned16(q_out) || !aligned16(cos_sin)) return NQB200_ERR_MISALIGNED;
+  const bool wide = row_stride % 8 == 0 && aligned16(qkv) && aligned16(q_weight) && aligned16(k_weight);
   StoreArgs a = {(const uint16_t*)qkv, row_stride, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos_sin, max_positions, positions, rows,
                  kv4::cache_of(cache), (uint16_t*)q_out, (int)T, (int)num_q_heads, eps, status};
   const int64_t heads = T * (num_q_heads + 2 * cache->kv_heads);
-  return launch_overlapped(dtype == NQB200_BF16 ? kv4_store_kernel<true> : kv4_store_kernel<false>, dim3((unsigned)((heads + 15) / 16)), dim3(256), 0,
+  const auto kernel = dtype == NQB200_BF16 ? (wide ? kv4_store_kernel<true, true> : kv4_store_kernel<true, false>) : (wide ? kv4_store_kernel<false, true> : kv4_store_kernel<false, false>);
+  return launch_overlapped(kernel, dim3((unsigned)((heads + 31) / 32)), dim3(256), 0,
                            (cudaStream_t)stream, a);
 }
 

@@ -29,61 +29,75 @@ def new_cache(num_blocks: int, block_size: int, kv_heads: int, device) -> tuple[
     return tuple(torch.zeros(num_blocks, kv_heads, block_size * TOKEN, dtype=torch.uint8, device=device) for _ in range(2))
 
 
+# Checks are written for few Python operations: a call of a few microseconds on the GPU is made as often as the host can make it.
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> _lib.Kv4:
-    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+    if k_cache.dtype is not torch.uint8 or v_cache.dtype is not torch.uint8:
         raise TypeError("a 4-bit cache is a pair of byte tensors")
-    if k_cache.dim() != 3 or k_cache.shape != v_cache.shape or k_cache.shape[2] % (16 * TOKEN) or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+    shape = k_cache.shape
+    if len(shape) != 3 or v_cache.shape != shape or shape[2] % (16 * TOKEN) or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError(f"a 4-bit cache is two contiguous tensors [pages, kv_heads, block_size * {TOKEN}] with blocks of a multiple of 16 tokens, got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    pages, heads, nbytes = k_cache.shape
-    return _lib.Kv4(k_cache.data_ptr(), v_cache.data_ptr(), pages, heads, nbytes // TOKEN)
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
+    return _lib.Kv4(k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[1], shape[2] // TOKEN)
 
 
 def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
-def _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, kv_heads, rows):
-    code = _lib.dtype_code(qkv.dtype)
-    if qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * kv_heads) * DIM or qkv.stride(1) != 1:
-        raise ValueError(f"qkv must be [tokens, {(num_q_heads + 2 * kv_heads) * DIM}] with unit stride along a row, got {tuple(qkv.shape)}")
+def _on_one_gpu(device: int, tensors: tuple) -> None:
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            _lib.require_cuda(*tensors)        # says what is wrong
+
+
+def _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, kv_heads, rows, cache):
+    """Checks of what a step's tokens come with; the type's code."""
+    dtype, shape = qkv.dtype, qkv.shape
+    if cache.kv_heads != kv_heads or num_q_heads % kv_heads:
+        raise ValueError(f"{num_q_heads} query heads over {kv_heads} do not go with a cache of {cache.kv_heads} key/value heads")
+    if len(shape) != 2 or shape[1] != (num_q_heads + 2 * kv_heads) * DIM or qkv.stride(1) != 1:
+        raise ValueError(f"qkv must be [tokens, {(num_q_heads + 2 * kv_heads) * DIM}] with unit stride along a row, got {tuple(shape)}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype != qkv.dtype or w.shape != (DIM,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {qkv.dtype} tensor of {DIM}")
-    if cos_sin.dtype != torch.float32 or cos_sin.shape[-1] != DIM or not cos_sin.is_contiguous():
+        if w.dtype is not dtype or w.shape != (DIM,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {DIM}")
+    if cos_sin.dtype is not torch.float32 or cos_sin.shape[-1] != DIM or not cos_sin.is_contiguous():
         raise ValueError(f"cos_sin must be a contiguous float32 tensor [..., {DIM}]")
-    _ints("positions", positions, torch.int64, (qkv.shape[0],))
-    _ints("rows", rows, torch.int64, (qkv.shape[0],))
-    return code
+    tokens = shape[:1]
+    _ints("positions", positions, torch.int64, tokens)
+    _ints("rows", rows, torch.int64, tokens)
+    return _lib.dtype_code(dtype)
 
 
 def qknorm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, num_q_heads: int,
                       num_kv_heads: int, eps: float, k_cache: torch.Tensor, v_cache: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
     """Per-head RMSNorm and rotary embedding of q and k in ``qkv [T, (Hq + 2 Hkv) * 128]`` (left as it is); k and v of token t are stored in
     cache row ``rows[t]`` (below 0: nowhere).  Returns the queries ``[T, Hq * 128]``."""
-    dev = _lib.require_cuda(qkv, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, rows)
+    dev = qkv.get_device()
+    _on_one_gpu(dev, (qkv, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, rows))
     cache = _cache(k_cache, v_cache)
-    if cache.kv_heads != num_kv_heads:
-        raise ValueError(f"the cache holds {cache.kv_heads} key/value heads, the projections {num_kv_heads}")
-    code = _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, num_kv_heads, rows)
-    T = qkv.shape[0]
-    out = torch.empty(T, num_q_heads * DIM, dtype=qkv.dtype, device=dev)
-    with _lib.on_device(dev) as on:
-        _lib.check(_lib.load().nqb200_kv4_store(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(),
-                                                cos_sin.numel() // DIM, positions.data_ptr(), rows.data_ptr(), cache, out.data_ptr(), T, num_q_heads,
-                                                float(eps), code, _lib.cache_status(on.index), on.stream))
+    code = _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, num_kv_heads, rows, cache)
+    with _lib.on_device(dev) as stream:
+        T = qkv.shape[0]
+        out = qkv.new_empty((T, num_q_heads * DIM))
+        status = _lib.load().nqb200_kv4_store(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM,
+                                              positions.data_ptr(), rows.data_ptr(), cache, out.data_ptr(), T, num_q_heads, eps, code,
+                                              _lib.cache_status(dev), stream)
+    _lib.check(status)
     return out
 
 
 def load(k_cache: torch.Tensor, v_cache: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of cache rows (int64; below 0: zeros) as ``[n, kv_heads, 128]`` of ``dtype``, the type they were written in."""
-    dev = _lib.require_cuda(k_cache, v_cache, rows)
+    dev = k_cache.get_device()
+    _on_one_gpu(dev, (k_cache, v_cache, rows))
     cache, code, n = _cache(k_cache, v_cache), _lib.dtype_code(dtype), rows.numel()
     _ints("rows", rows, torch.int64, (n,))
-    k, v = (torch.empty(n, cache.kv_heads, DIM, dtype=dtype, device=dev) for _ in range(2))
-    with _lib.on_device(dev) as on:
-        _lib.check(_lib.load().nqb200_kv4_load(cache, rows.data_ptr(), k.data_ptr(), v.data_ptr(), n, code, _lib.cache_status(on.index), on.stream))
+    with _lib.on_device(dev) as stream:
+        shape = (n, cache.kv_heads, DIM)
+        k, v = k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+        status = _lib.load().nqb200_kv4_load(cache, rows.data_ptr(), k.data_ptr(), v.data_ptr(), n, code, _lib.cache_status(dev), stream)
+    _lib.check(status)
     return k, v
 
 
@@ -92,23 +106,23 @@ def decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.
                      scale: float | None = None) -> torch.Tensor:
     """One token per sequence: what ``qknorm_rope_store`` does to it, then attention over the ``ctx[b]`` keys (int32) of sequence b, its
     own among them, whose pages are ``table[b]`` (int32).  ``ctx[b] = 0``: a row without a sequence, which gets zeros.  Returns ``[B, Hq * 128]``."""
-    dev = _lib.require_cuda(qkv, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, table, ctx, rows)
+    dev = qkv.get_device()
+    _on_one_gpu(dev, (qkv, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, table, ctx, rows))
     cache = _cache(k_cache, v_cache)
-    if cache.kv_heads != num_kv_heads or num_q_heads % num_kv_heads:
-        raise ValueError(f"{num_q_heads} query heads over {num_kv_heads} do not go with a cache of {cache.kv_heads} key/value heads")
-    code = _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, num_kv_heads, rows)
+    code = _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, num_kv_heads, rows, cache)
     B, width = qkv.shape[0], table.shape[-1]
     _ints("table", table, torch.int32, (B, width))
     _ints("ctx", ctx, torch.int32, (B,))
-    out = torch.empty(B, num_q_heads * DIM, dtype=qkv.dtype, device=dev)
     lib = _lib.load()
-    with _lib.on_device(dev) as on:
+    with _lib.on_device(dev) as stream:
+        out = qkv.new_empty((B, num_q_heads * DIM))
         need = lib.nqb200_kv4_decode_scratch_bytes(width, cache.block_size, B, num_q_heads, num_kv_heads)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.nqb200_kv4_decode_attention(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(),
-                                                   cos_sin.numel() // DIM, positions.data_ptr(), rows.data_ptr(), cache, table.data_ptr(), width,
-                                                   ctx.data_ptr(), out.data_ptr(), B, num_q_heads, DIM ** -0.5 if scale is None else float(scale), float(eps),
-                                                   code, scratch.data_ptr() if need else None, need, _lib.cache_status(on.index), on.stream))
+        scratch = k_cache.new_empty(need) if need else None
+        status = lib.nqb200_kv4_decode_attention(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM,
+                                                 positions.data_ptr(), rows.data_ptr(), cache, table.data_ptr(), width, ctx.data_ptr(), out.data_ptr(), B,
+                                                 num_q_heads, DIM ** -0.5 if scale is None else scale, eps, code, scratch.data_ptr() if need else None, need,
+                                                 _lib.cache_status(dev), stream)
+    _lib.check(status)
     return out
 
 
@@ -117,24 +131,27 @@ def prompt_attention(q: torch.Tensor, num_q_heads: int, k_cache: torch.Tensor, v
     """Causal attention of several tokens per sequence over the cache, where their own keys and values have been stored already:
     ``q [T, Hq * 128]`` (normed and rotated) holds tokens ``cu[b] .. cu[b + 1] - 1`` of sequence b, at its positions ``pos0[b] ..`` (both int32);
     ``lens`` and ``starts`` are the same on the host.  Whole prompts, later portions and drafted tokens alike; returns ``[T, Hq * 128]``."""
-    dev = _lib.require_cuda(q, k_cache, v_cache, table, cu, pos0)
+    dev = q.get_device()
+    _on_one_gpu(dev, (q, k_cache, v_cache, table, cu, pos0))
     cache, code = _cache(k_cache, v_cache), _lib.dtype_code(q.dtype)
-    B, T, width = len(lens), q.shape[0], table.shape[-1]
-    if q.dim() != 2 or q.shape[1] != num_q_heads * DIM or q.stride(1) != 1 or num_q_heads % cache.kv_heads:
-        raise ValueError(f"q must be [tokens, {num_q_heads * DIM}] with unit stride along a row, the heads a multiple of the cache's {cache.kv_heads}; got {tuple(q.shape)}")
+    B, shape, width = len(lens), q.shape, table.shape[-1]
+    if len(shape) != 2 or shape[1] != num_q_heads * DIM or q.stride(1) != 1 or num_q_heads % cache.kv_heads:
+        raise ValueError(f"q must be [tokens, {num_q_heads * DIM}] with unit stride along a row, the heads a multiple of the cache's {cache.kv_heads}; got {tuple(shape)}")
+    T = shape[0]
     if len(starts) != B or sum(lens) != T or min(lens, default=0) < 0 or min(starts, default=0) < 0:
         raise ValueError(f"lens and starts must name the {T} tokens of q, one number each per sequence and none negative")
     _ints("table", table, torch.int32, (B, width))
     _ints("cu", cu, torch.int32, (B + 1,))
     _ints("pos0", pos0, torch.int32, (B,))
-    out = torch.empty(T, num_q_heads * DIM, dtype=q.dtype, device=dev)
     ends = [n + s for n, s in zip(lens, starts) if n]
-    max_len, max_ctx, tiles = max(lens, default=0), max(ends, default=0), sum(-(-e // TILE) for e in ends)
+    max_len, max_ctx, tiles = max(lens, default=0), max(ends, default=0), sum([(e + TILE - 1) // TILE for e in ends])
     lib = _lib.load()
-    with _lib.on_device(dev) as on:
+    with _lib.on_device(dev) as stream:
+        out = q.new_empty((T, num_q_heads * DIM))
         need = lib.nqb200_kv4_prompt_scratch_bytes(B, T, max_len, max_ctx, tiles, num_q_heads, cache.kv_heads)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.nqb200_kv4_prompt_attention(q.data_ptr(), q.stride(0), cache, table.data_ptr(), width, cu.data_ptr(), pos0.data_ptr(), out.data_ptr(), B, T,
-                                                   max_len, max_ctx, tiles, num_q_heads, DIM ** -0.5 if scale is None else float(scale), code,
-                                                   scratch.data_ptr() if need else None, need, _lib.cache_status(on.index), on.stream))
+        scratch = k_cache.new_empty(need) if need else None
+        status = lib.nqb200_kv4_prompt_attention(q.data_ptr(), q.stride(0), cache, table.data_ptr(), width, cu.data_ptr(), pos0.data_ptr(), out.data_ptr(), B, T, max_len,
+                                                 max_ctx, tiles, num_q_heads, DIM ** -0.5 if scale is None else scale, code, scratch.data_ptr() if need else None,
+                                                 need, _lib.cache_status(dev), stream)
+    _lib.check(status)
     return out
