@@ -111,9 +111,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 // A query as the first product's second operand, in units of a power of two that puts its largest element between 256 and 512: eight
-// lanes, as for head_values(); elements that meet 1024 + 16 n are divided by 16.  Returns the unit.
-__device__ __forceinline__ float operand(const float (&x)[8], const float (&y)[8], uint4& lo, uint4& hi) {
-  float top = 0.f;
+// lanes, as in kv4.cuh; elements that meet 1024 + 16 n are divided by 16.  Returns the unit.
+__device__ __forceinline__ float operand(const Half& hx, const Half& hy, uint4& lo, uint4& hi) {
+  float x[8], y[8], top = 0.f;
+  values(hx, x);
+  values(hy, y);
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
 #pragma unroll
@@ -234,19 +236,21 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   // queries into fx.q, eight lanes each: the first two warps; the step's own key and value: the third
   const int unit = tid >> 3, m8 = tid & 7;
   if (keys > 0 && (warp < 2 || (newest && warp == 2))) {
-    float x[8], y[8];
     const int c = min(unit, cols - 1), idx = group * kCols + c;      // (columns beyond `cols` repeat the last one and are not used)
     const bool is_v = unit == 9;
+    const uint16_t* src = DECODE ? a.q + (int64_t)b * a.stride + (int64_t)(warp < 2 ? kvh * R + idx : a.heads + (is_v ? a.cache.kv_heads : 0) + kvh) * kDim
+                                 : a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim;
+    const uint4 rx = fetch8<true>(src, m8), ry = fetch8<true>(src, m8 + 8);
+    Half x = unpack8<BF16>(rx), y = unpack8<BF16>(ry);
     if (DECODE) {
+      const uint16_t* weight = warp < 2 ? a.qw : a.kw;
+      const uint4 wx = fetch8<true>(weight, m8), wy = fetch8<true>(weight, m8 + 8);
       int64_t pos = a.positions[b];
       if (pos < 0 || pos >= a.max_positions) {
         if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
         pos = 0;
       }
-      const int head = warp < 2 ? kvh * R + idx : a.heads + (is_v ? a.cache.kv_heads : 0) + kvh;
-      head_values<BF16>(a.q + (int64_t)b * a.stride + (int64_t)head * kDim, warp < 2 ? a.qw : is_v ? nullptr : a.kw, a.cos_sin + pos * kDim, a.eps, x, y);
-    } else {
-      head_values<BF16>(a.q + (int64_t)(t_first + idx / R) * a.stride + (int64_t)(kvh * R + idx % R) * kDim, nullptr, nullptr, 0.f, x, y);
+      norm_turn<BF16>(x, y, wx, wy, angles_of(a.cos_sin + pos * kDim), a.eps, !is_v);
     }
     if (warp < 2) {
       uint4 lo, hi;

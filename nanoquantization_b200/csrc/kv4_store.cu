@@ -22,7 +22,7 @@ struct StoreArgs {
 };
 
 template <bool BF16, bool WIDE>
-__global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ StoreArgs a) {
+__global__ void __launch_bounds__(256, 5) kv4_store_kernel(const __grid_constant__ StoreArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int m = threadIdx.x & 7, Hq = a.heads, Hkv = a.cache.kv_heads, per = Hq + 2 * Hkv;
@@ -31,12 +31,14 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   const int t = in ? at / per : 0, hd = in ? at - t * per : 0;
   const bool is_v = hd >= Hq + Hkv, is_q = hd < Hq;
   int64_t pos = a.positions[t];
+  const uint16_t *src = a.qkv + (int64_t)t * a.stride + (int64_t)hd * kDim, *weight = is_q ? a.qw : a.kw;
+  const uint4 rx = fetch8<WIDE>(src, m), ry = fetch8<WIDE>(src, m + 8);
   if (pos < 0 || pos >= a.max_positions) {
     if (in && hd == 0 && m == 0) report(a.status, NQB200_ERR_BAD_INDEX);
     pos = 0;
   }
-  float x[8], y[8];
-  head_values<BF16, WIDE>(a.qkv + (int64_t)t * a.stride + (int64_t)hd * kDim, is_v ? nullptr : is_q ? a.qw : a.kw, a.cos_sin + pos * kDim, a.eps, x, y);
+  Half x = unpack8<BF16>(rx), y = unpack8<BF16>(ry);
+  norm_turn<BF16>(x, y, fetch8<WIDE>(weight, m), fetch8<WIDE>(weight, m + 8), angles_of(a.cos_sin + pos * kDim), a.eps, !is_v);
   if (__any_sync(0xFFFFFFFFu, in && !is_q)) {          // (a warp's other heads go along)
     uint2 words, params;
     quantise<BF16>(x, y, words, params);
@@ -54,9 +56,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   }
   if (in && is_q) {
     uint4* dst = reinterpret_cast<uint4*>(a.q_out + ((int64_t)t * Hq + hd) * kDim);
-    const auto pack = [](float p, float q) { return (uint32_t)float_to_raw16<BF16>(p) | ((uint32_t)float_to_raw16<BF16>(q) << 16); };
-    dst[m] = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
-    dst[m + 8] = make_uint4(pack(y[0], y[1]), pack(y[2], y[3]), pack(y[4], y[5]), pack(y[6], y[7]));
+    dst[m] = pack8<BF16>(x);
+    dst[m + 8] = pack8<BF16>(y);
   }
 }
 
