@@ -1,16 +1,18 @@
 // Attention over the 4-bit key/value cache for many queries: prompts and their portions, on the 5th-generation tensor cores.
 //
-// Two launches.  The first takes the visible pages apart, once, into tiles of 128 keys and 128 values in the 16-bit type, each 32 KB as the tensor
+// Two launches.  The first takes the visible pages apart, once, into tiles of 128 keys and 128 values in float16, each 32 KB as the tensor
 // cores want it in shared memory (blocks of 64 dimensions, rows of 128 bytes, swizzled), so that the second fetches a tile with one bulk copy
-// and needs no tensor map.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the first of
-// those stands is noted, and the rows that see it get NaN at the end, and no other (a weight of 0 times NaN would be one).
+// and needs no tensor map.  float16 whatever the model's type: keys, values and weights in bfloat16 cost twice the error of the
+// result's own rounding (a prompt of 8000 tokens: 0.0031 in the 2-norm, 0.0017 so).  A tile whose numbers float16 would not hold well is in units of a
+// power of two, and so is a query.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the
+// first of those stands is noted, and the rows that see it get NaN at the end, and no other (a weight of 0 times NaN would be one).
 //
 // In the second a CTA takes 256 rows of a key/value head, as two tiles of 128: a row is a query head of a token, the heads of a group beside
 // each other, so that the mask cuts as few tiles as it can and short prompts fill a tile.  It walks over tiles of 128 keys, each in two halves of 64.
 //   warp 0        copies: two-stage rings of K tiles and of V tiles.
 //   warps 1, 2    one lane of each issues tcgen05.mma for a query tile: S = Q K^T of a half (both operands in shared memory)
 //                 and O += P V (P in tensor memory, V in shared memory as it lies there: the operand's rows are keys).
-//   warp 3        looks for values that are not finite.
+//   warp 3        looks for tiles in other units than 1, and for values that are not finite.
 //   warps 4-19    softmax: four warps for each half of each query tile, a thread per row and half.
 // Tensor memory holds S of both tiles (two halves of 64 columns each) and O of both; P overwrites the first half of its own S.  So four
 // chains S -> weights -> O += P V -> next S run beside each other.
@@ -40,6 +42,21 @@ constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLag = 7.f;
 constexpr int kNone = 0x7FFFFFFF;
 
+struct alignas(16) TileInfo {
+  int bad[2];            // the tile's first key whose value is not finite in dimensions 0..63, in 64..127, or kNone
+  float k, v;            // units of the tile's keys and values
+};
+// The unit of numbers up to `top`: 1 where float16 holds them well, else the power of two that puts `top` between 2^13 and 2^14.
+__device__ __forceinline__ float unit_of(float top) {
+  if (top == 0.f || (top >= 0.015625f && top < 32768.f)) return 1.f;
+  const uint32_t e = min(max(__float_as_uint(top) >> 23, 15u), 254u);
+  return __uint_as_float((e - 13u) << 23);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 struct Params {
   const uint16_t* q; int64_t q_stride;
   Cache cache;
@@ -47,11 +64,11 @@ struct Params {
   const int32_t *cu, *pos0;
   uint16_t* out;
   uint8_t* tiles;        // [tile of a sequence][kv head][K, V][kTileBytes]
-  int2* bad;             // [tile][kv head]: the first key of the tile whose value is not finite in dimensions 0..63, in 64..127, or kNone
+  TileInfo* info;        // [tile][kv head]
   float* shares;
   int heads, tokens, batch, parts, max_len, max_ctx, total;     // total: tiles that there is room for
   float factor;          // scale log2 e, not negative
-  uint32_t flip;         // 0x80008000 where the scale is negative: the queries change their sign
+  float sign;            // of the scale: the queries take it
   int* status;
 };
 
@@ -77,6 +94,7 @@ __device__ __forceinline__ int tiles_before(const Params& p, int b) {
 template <bool BF16>
 __global__ void __launch_bounds__(512) kv4_expand_kernel(const __grid_constant__ Params p) {
   __shared__ int s_before, s_bad[2];
+  __shared__ uint32_t s_top[2];
   grid_launch_dependents();
   grid_dependency_wait();
   const int b = blockIdx.z, h = blockIdx.y, tile = blockIdx.x, lane = threadIdx.x & 15;
@@ -87,7 +105,7 @@ __global__ void __launch_bounds__(512) kv4_expand_kernel(const __grid_constant__
   }
   const int key0 = tile * kTileKeys;
   if (key0 >= s.keys) return;
-  if (threadIdx.x < 2) s_bad[threadIdx.x] = kNone;
+  if (threadIdx.x < 2) { s_bad[threadIdx.x] = kNone; s_top[threadIdx.x] = 0u; }
   if (threadIdx.x < 32) {
     const int before = tiles_before(p, b);
     if (threadIdx.x == 0) s_before = before;
@@ -100,33 +118,58 @@ __global__ void __launch_bounds__(512) kv4_expand_kernel(const __grid_constant__
   }
   uint8_t* dst = p.tiles + (at * p.cache.kv_heads + h) * (2 * (int64_t)kTileBytes);
   const int j = lane & 1, m = lane >> 1;
+  constexpr int kPer = kTileKeys / 32;          // rows of a thread
+  uint32_t word[2][kPer], params[2][kPer];
+  bool there[kPer];
+  float top[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kTileKeys / 32; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const int r = i * 32 + (threadIdx.x >> 4), key = key0 + r, blk = key / p.cache.block;
     const int page = key < s.keys ? p.table[(int64_t)b * p.width + blk] : 0;
-    const bool there = key < s.keys && page >= 0 && page < p.cache.pages;
-    if (key < s.keys && !there && lane == 0) report(p.status, NQB200_ERR_BAD_INDEX);
-    const int64_t base = there ? page_at(p.cache, page, h) : 0, row = key - (int64_t)blk * p.cache.block, par = base + (int64_t)p.cache.block * kData + row * kParams + 4 * j;
+    there[i] = key < s.keys && page >= 0 && page < p.cache.pages;
+    if (key < s.keys && !there[i] && lane == 0) report(p.status, NQB200_ERR_BAD_INDEX);
+    const int64_t base = there[i] ? page_at(p.cache, page, h) : 0, row = there[i] ? key - (int64_t)blk * p.cache.block : 0;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const uint8_t* c = which ? p.cache.v : p.cache.k;
-      uint32_t out[4] = {0u, 0u, 0u, 0u};
-      if (there) {
-        const uint32_t word = reinterpret_cast<const uint32_t*>(c + base + row * kData)[lane], params = *reinterpret_cast<const uint32_t*>(c + par);
-        const float sc = scale_of<BF16>(params), off = offset_of<BF16>(params);
-        const bool fine = fabsf(sc) < INFINITY && fabsf(off) < INFINITY;
-        if (which && !fine) {
-          atomicMin(&s_bad[j], key);
-        } else {
+      const uint8_t* c = (which ? p.cache.v : p.cache.k) + base;
+      word[which][i] = reinterpret_cast<const uint32_t*>(c + row * kData)[lane];
+      params[which][i] = *reinterpret_cast<const uint32_t*>(c + (int64_t)p.cache.block * kData + row * kParams + 4 * j);
+    }
+  }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[e] = (uint32_t)level<BF16>(nibble(word, e), sc, off) | ((uint32_t)level<BF16>(nibble(word, e + 4), sc, off) << 16);
-        }
+  for (int i = 0; i < kPer; ++i) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const float sc = scale_of<BF16>(params[which][i]), off = offset_of<BF16>(params[which][i]), most = max_nan(fabsf(off), fabsf(fmaf(15.f, sc, off)));
+      if (there[i] && most < INFINITY) {
+        top[which] = fmaxf(top[which], most);
+      } else if (there[i] && which) {
+        atomicMin(&s_bad[j], key0 + i * 32 + (int)(threadIdx.x >> 4));
       }
+    }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top[which]));
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_top[which], all);
+  }
+  __syncthreads();
+  const float unit[2] = {unit_of(__uint_as_float(s_top[0])), unit_of(__uint_as_float(s_top[1]))};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const float by = 1.f / unit[which];         // a power of two
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = i * 32 + (threadIdx.x >> 4);
+      const float sc = scale_of<BF16>(params[which][i]) * by, off = offset_of<BF16>(params[which][i]) * by;
+      const bool zero = !there[i] || (which && !(max_nan(fabsf(off), fabsf(fmaf(15.f, sc, off))) < INFINITY));
+      uint32_t out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = zero ? 0u : pack_half(fmaf(nibble(word[which][i], e), sc, off), fmaf(nibble(word[which][i], e + 4), sc, off));
       *reinterpret_cast<uint4*>(dst + which * kTileBytes + j * kBox + r * 128 + ((m ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
-  __syncthreads();
-  if (threadIdx.x == 0) p.bad[at * p.cache.kv_heads + h] = make_int2(s_bad[0], s_bad[1]);
+  if (threadIdx.x == 0) p.info[at * p.cache.kv_heads + h] = TileInfo{{s_bad[0], s_bad[1]}, unit[0], unit[1]};
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -145,7 +188,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   __shared__ __align__(8) uint64_t bar_kfull[2], bar_kfree[2], bar_vfull[2], bar_vfree[2], bar_s[2][2], bar_p[2][2], bar_pv[2][2], bar_o[2], bar_x[2][4], bar_m[2][2][4], bar_bad, bar_drain;
   __shared__ float s_x[2][2][2][128], s_m[2][2][128];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort_i, s_before, s_bad[2];
+  __shared__ int s_abort_i, s_before, s_bad[2], s_special;
+  __shared__ float s_row[kRows], s_unit_v;     // units of the queries; the largest of the values'
   volatile int* s_abort = &s_abort_i;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem_q = smem_raw + (smem - smem_u32(smem_raw));
@@ -189,11 +233,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     if (lane == 0) s_before = before;
   }
   // the queries, 16 lanes a row: block of 64 dimensions, row of 128 bytes, piece swizzled by the row
-  for (int i = threadIdx.x >> 4; i < kRows; i += kThreads / 16) {
+  for (int i = threadIdx.x >> 4; i < kRows; i += kThreads / 16) {      // (a warp's two rows alike: 40 warps' halves, 256 rows)
     const int row = i0 + i, l = threadIdx.x & 15;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows) v = reinterpret_cast<const uint4*>(p.q + (int64_t)(sp.first + row / R) * p.q_stride + (int64_t)(kvh * R + row % R) * kDim)[l];
-    v.x ^= p.flip; v.y ^= p.flip; v.z ^= p.flip; v.w ^= p.flip;
+    float x[8], top = 0.f;
+    values(unpack8<BF16>(v), x);
+    if (BF16) {                        // (float16 goes in as it is)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    }
+    const float unit = BF16 ? unit_of(top) : 1.f, by = p.sign / unit;
+    v = make_uint4(pack_half(x[0] * by, x[1] * by), pack_half(x[2] * by, x[3] * by), pack_half(x[4] * by, x[5] * by), pack_half(x[6] * by, x[7] * by));
+    if (l == 0) s_row[i] = unit;
     *reinterpret_cast<uint4*>(smem_q + (i >> 7) * kQBytes + (l >> 3) * kBox + (i & 127) * 128 + (((l & 7) ^ (i & 7)) << 4)) = v;
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the tensor cores read them
@@ -201,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int64_t tile0 = (int64_t)s_before + first;                 // of the scratch
+  const int tile0 = s_before + first;                              // of the scratch
   const bool fits = tile0 + nmax <= p.total;                       // (the first launch has reported it)
   if (!fits) nq[0] = nq[1] = 0;
   const int n_tiles = fits ? nmax : 0;
@@ -214,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     int issued = 0;
     for (int j = 0; j < n_tiles; ++j, ++issued) {
       const int s = j & 1;
-      const uint8_t* src = p.tiles + ((tile0 + j) * p.cache.kv_heads + kvh) * (2 * (int64_t)kTileBytes);
+      const uint8_t* src = p.tiles + ((int64_t)(tile0 + j) * p.cache.kv_heads + kvh) * (2 * (int64_t)kTileBytes);
       if (j >= 2 && !wait_bar_warp(&bar_kfree[s], ((j >> 1) - 1) & 1, s_abort, p.status)) break;
       if (el) {
         mbar_expect_tx(smem_u32(&bar_kfull[s]), kTileBytes);
@@ -240,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     // completed.  A ring stage is handed back by both warps, by its only user twice.
     const int q = warp - 1;
     const bool el = elect_one();
-    const uint32_t idesc_s = umma_idesc(BF16 ? 1 : 0, 128, kTileKeys / 2);
-    const uint32_t idesc_o = umma_idesc(BF16 ? 1 : 0, 128, kDim) | (1u << 16);   // B's rows run along k
+    const uint32_t idesc_s = umma_idesc(0, 128, kTileKeys / 2);
+    const uint32_t idesc_o = umma_idesc(0, 128, kDim) | (1u << 16);   // B's rows run along k
     const uint64_t dq = umma_smem_desc_sw128(smem + q * kQBytes), dk = umma_smem_desc_sw128(smem + kOffK), dv = smem_desc_mn(smem + kOffV, kBox);
     const uint32_t k_hi = (uint32_t)(dq >> 32), v_hi = (uint32_t)(dv >> 32), q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, v_lo = (uint32_t)dv;
     const uint32_t tS = tmem + kColS + q * 128, tO = tmem + kColO + q * 128;
@@ -291,25 +345,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     if (el) umma_commit(smem_u32(&bar_drain));
     mbar_wait(smem_u32(&bar_drain), 0);
   } else if (warp == 3) {
-    // ------------------------------------------------ values that are not finite
+    // ------------------------------------------------ units, and values that are not finite
     int low[2] = {kNone, kNone};
+    uint32_t unit_v = 0u;
+    bool special = false;
     for (int j = lane; j < n_tiles; j += 32) {
-      const int2 v = p.bad[(tile0 + j) * p.cache.kv_heads + kvh];
-      low[0] = min(low[0], v.x);
-      low[1] = min(low[1], v.y);
+      const TileInfo v = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y];
+      low[0] = min(low[0], v.bad[0]);
+      low[1] = min(low[1], v.bad[1]);
+      unit_v = max(unit_v, __float_as_uint(v.v));
+      special = special || v.k != 1.f || v.v != 1.f;
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g) low[g] = __reduce_min_sync(0xFFFFFFFFu, low[g]);
+    unit_v = __reduce_max_sync(0xFFFFFFFFu, unit_v);
+    special = __any_sync(0xFFFFFFFFu, special);
     if (lane == 0) {
       s_bad[0] = low[0];
       s_bad[1] = low[1];
+      s_unit_v = __uint_as_float(unit_v);
+      s_special = special;
       mbar_arrive(smem_u32(&bar_bad));
     }
   } else {
     // -------------------------------------------------------------- softmax
     const int q = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16, tS = tmem + lanes + kColS + q * 128 + half * 64, tO = tmem + lanes + kColO + q * 128;
-    const int i = i0 + q * 128 + row, pos = pos_of(i), wfirst = pos_of(i - lane);
+    const int i = i0 + q * 128 + row, pos = pos_of(i);
     auto done = [&]() {           // this half of the weights is in tensor memory
       tc_wait_st();
       tc_fence_before();
@@ -329,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       ++exchanges;
       return got;
     };
+    const float row_factor = BF16 ? p.factor * s_row[q * 128 + row] : p.factor;
     float m = -INFINITY;
     uint64_t lsum = pair2(0.f, 0.f);
     // A row's reference goes from half to half in the order of their products: 0 and 1 of the first tile, 0 and 1 of the next, and so on,
@@ -351,14 +414,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       if (half == 1) return j == 0 || take(j);
       return j < 2 || take(j - 1);
     };
-    bool ok = true;
-    for (int j = 0; j < nq[q]; ++j) {
+    bool ok = wait_bar_warp(&bar_bad, 0, s_abort, p.status);
+    // the first position of the warp; with tiles in other units every tile takes the general way
+    const int wfirst = s_special ? -1 : pos_of(i - lane);
+    for (int j = 0; ok && j < nq[q]; ++j) {
       const bool joint = j == 0;
       ok = catch_up(j) && wait_bar_warp(&bar_s[q][half], j & 1, s_abort, p.status);
       if (!ok) break;
       tc_fence_after();
       const int key0 = kstart + j * kTileKeys + half * 64;
       const bool masked = key0 + 63 > wfirst;     // for any row of the warp
+      float factor = row_factor;
+      if (masked && s_special) factor *= p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].k;
       uint32_t r[2][32];     // the row's scores, all of this half
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld32(tS + c * 32, r[c]);
@@ -374,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ab = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
       }
       const float lag = m + kLag;
-      if (joint || masked || !__all_sync(0xFFFFFFFFu, ab * p.factor <= lag)) {
+      if (joint || masked || !__all_sync(0xFFFFFFFFu, ab * factor <= lag)) {
         if (!masked) {
           float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -393,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
           if (!(ok = exchange(mx, mo))) break;
           mx = fmaxf(mx, mo);
         }
-        mx = mx == -INFINITY ? mx : mx * p.factor;
+        mx = mx == -INFINITY ? mx : mx * factor;
       }
       const bool move = mx > lag;      // also from -inf
       if (!joint) pass(move ? mx : m);
@@ -419,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         tc_wait_ld();
       }
       const float mu = m == -INFINITY ? 0.f : m;
-      const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(p.factor, p.factor);
+      const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(factor, factor);
       if (!masked) {
         uint64_t ls[2] = {lsum, 0};
 #pragma unroll
@@ -431,14 +498,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             unpair2(fma2(pair2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), k1, nm2), x0, x1);
             x0 = ex2(x0);
             x1 = ex2(x1);
-            w[e] = pack16<BF16>(x0, x1);
+            w[e] = pack_half(x0, x1);
             ls[e & 1] = add2(ls[e & 1], pair2(x0, x1));
           }
           tmem_st16(tS + c * 16, w);
         }
         lsum = add2(ls[0], ls[1]);
       } else {
-        // from tensor memory again, a piece at a time: compact code for the few tiles at the edge
+        // from tensor memory again, a piece at a time: compact code for the few tiles at the edge, and for sequences with tiles in other units
+        const float by = s_special ? p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].v / s_unit_v : 1.f;      // of the tile's weights in the product
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t v[16], w[8];
@@ -448,8 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
           for (int e = 0; e < 8; ++e) {
             float x[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) x[u] = key0 + c * 16 + 2 * e + u <= pos ? ex2(fmaf(__uint_as_float(v[2 * e + u]), p.factor, -mu)) : 0.f;
-            w[e] = pack16<BF16>(x[0], x[1]);
+            for (int u = 0; u < 2; ++u) x[u] = key0 + c * 16 + 2 * e + u <= pos ? ex2(fmaf(__uint_as_float(v[2 * e + u]), factor, -mu)) : 0.f;
+            w[e] = pack_half(x[0] * by, x[1] * by);
             lsum = add2(lsum, pair2(x[0], x[1]));
           }
           tmem_st8(tS + c * 8, w);      // lies behind what has been read of S
@@ -457,8 +525,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       }
       done();
     }
-    const int64_t out_row = (int64_t)(sp.first + min(i, rows - 1) / R) * p.heads + kvh * R + min(i, rows - 1) % R;
-    float* share = p.shares + (out_row * p.parts + part) * kShare + half * 64;
+    const int R = p.heads / p.cache.kv_heads, at = min(i, span_of(p, blockIdx.z).n * R - 1);      // (again, rather than in registers until here)
+    const int64_t out_row = (int64_t)(p.cu[blockIdx.z] + at / R) * p.heads + blockIdx.y * R + at % R;
+    const bool mine = at == i;
+    float* share = p.shares + (out_row * p.parts + blockIdx.x % p.parts) * kShare + half * 64;
     if (ok && nq[q] > 0) {
       ok = (half == 1 || catch_up(nq[q])) && wait_bar_warp(&bar_o[q], 0, s_abort, p.status);
       float l = 0.f;
@@ -469,24 +539,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         ok = exchange(l, other);
         l += other;
       }
-      ok = ok && wait_bar_warp(&bar_bad, 0, s_abort, p.status);
       if (ok) {
         tc_fence_after();
         // dimensions 64 half ..: NaN where a value that the row sees is none
         const float poison = s_bad[half] <= pos ? __int_as_float(0x7FC00000) : 0.f;
-        const float f = p.parts > 1 ? 1.f : 1.f / l;
+        const float f = p.parts > 1 ? s_unit_v : s_unit_v / l;
         uint16_t* dst = p.out + out_row * kDim + half * 64;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t r[32];
           tmem_ld32(tO + half * 64 + c * 32, r);
           tc_wait_ld();
-          if (i < rows) {
+          if (mine) {
             if (p.parts > 1) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(share + c * 32 + e * 4) = make_float4(__uint_as_float(r[4 * e]) + poison, __uint_as_float(r[4 * e + 1]) + poison,
-                                                                                  __uint_as_float(r[4 * e + 2]) + poison, __uint_as_float(r[4 * e + 3]) + poison);
+                *reinterpret_cast<float4*>(share + c * 32 + e * 4) =
+                    make_float4(fmaf(__uint_as_float(r[4 * e]), f, poison), fmaf(__uint_as_float(r[4 * e + 1]), f, poison),
+                                fmaf(__uint_as_float(r[4 * e + 2]), f, poison), fmaf(__uint_as_float(r[4 * e + 3]), f, poison));
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -501,13 +571,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
           }
           __syncwarp();
         }
-        if (p.parts > 1 && i < rows && half == 0) { share[kDim] = m; share[kDim + 1] = l; }
+        if (p.parts > 1 && mine && half == 0) { share[kDim] = m; share[kDim + 1] = l; }
         tc_fence_before();
       }
-    } else if (nq[q] == 0 && p.parts > 1 && i < rows) {      // no keys of this part, or none that could be read
+    } else if (nq[q] == 0 && p.parts > 1 && mine) {      // no keys of this part, or none that could be read
       for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(share + e * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
       if (half == 0) { share[kDim] = -INFINITY; share[kDim + 1] = 0.f; }
-    } else if (nq[q] == 0 && i < rows) {
+    } else if (nq[q] == 0 && mine) {
       for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(p.out + out_row * kDim + half * 64 + e * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
@@ -518,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 }
 
 int64_t tile_bytes(int64_t tiles, int64_t kv_heads) { return tiles * kv_heads * 2 * (int64_t)kTileBytes; }
-int64_t bad_bytes(int64_t tiles, int64_t kv_heads) { return (tiles * kv_heads * (int64_t)sizeof(int2) + 15) / 16 * 16; }
+int64_t info_bytes(int64_t tiles, int64_t kv_heads) { return tiles * kv_heads * (int64_t)sizeof(TileInfo); }
 
 // CTAs that a row tile's keys are dealt to: as many as fill the SMs, with at least four tiles of keys each.
 int parts_of(int64_t batch, int64_t max_len, int64_t max_ctx, int64_t heads, int64_t kv_heads) {
@@ -535,7 +605,7 @@ bool prompt_umma_supports(int64_t batch, int64_t tokens, int64_t max_len, int64_
 }
 size_t prompt_umma_scratch_bytes(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
   const int parts = parts_of(batch, max_len, max_ctx, heads, kv_heads);
-  return (size_t)(tile_bytes(tiles, kv_heads) + bad_bytes(tiles, kv_heads) + (parts > 1 ? tokens * heads * parts * kShare * (int64_t)sizeof(float) : 0));
+  return (size_t)(tile_bytes(tiles, kv_heads) + info_bytes(tiles, kv_heads) + (parts > 1 ? tokens * heads * parts * kShare * (int64_t)sizeof(float) : 0));
 }
 int prompt_umma(const uint16_t* q, int64_t q_stride, const nqb200_kv4* cache, const int32_t* table, int64_t width, const int32_t* cu, const int32_t* pos0,
                 uint16_t* out, int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, float scale, int dtype, void* scratch,
@@ -543,10 +613,10 @@ int prompt_umma(const uint16_t* q, int64_t q_stride, const nqb200_kv4* cache, co
   Params p = {};
   const int64_t hk = cache->kv_heads;
   p.q = q; p.q_stride = q_stride; p.cache = cache_of(cache); p.table = table; p.width = width; p.cu = cu; p.pos0 = pos0; p.out = out;
-  p.tiles = (uint8_t*)scratch; p.bad = (int2*)(p.tiles + tile_bytes(tiles, hk)); p.shares = (float*)((uint8_t*)p.bad + bad_bytes(tiles, hk));
+  p.tiles = (uint8_t*)scratch; p.info = (TileInfo*)(p.tiles + tile_bytes(tiles, hk)); p.shares = (float*)((uint8_t*)p.info + info_bytes(tiles, hk));
   p.heads = (int)heads; p.tokens = (int)tokens; p.batch = (int)batch; p.max_len = (int)max_len; p.max_ctx = (int)max_ctx; p.total = (int)tiles;
   p.parts = parts_of(batch, max_len, max_ctx, heads, hk);
-  p.factor = fabsf(scale) * kLog2e; p.flip = scale < 0.f ? 0x80008000u : 0u; p.status = status;
+  p.factor = fabsf(scale) * kLog2e; p.sign = scale < 0.f ? -1.f : 1.f; p.status = status;
   const bool bf16 = dtype == NQB200_BF16;
   const dim3 expand((unsigned)((max_ctx + kTileKeys - 1) / kTileKeys), (unsigned)hk, (unsigned)batch);
   int rc = launch_overlapped(bf16 ? kv4_expand_kernel<true> : kv4_expand_kernel<false>, expand, dim3(512), 0, st, p);
