@@ -231,24 +231,37 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   if (warp == 0) {
     const int before = tiles_before(p, b);
     if (lane == 0) s_before = before;
-  }
-  // the queries, 16 lanes a row: block of 64 dimensions, row of 128 bytes, piece swizzled by the row
-  for (int i = threadIdx.x >> 4; i < kRows; i += kThreads / 16) {      // (a warp's two rows alike: 40 warps' halves, 256 rows)
-    const int row = i0 + i, l = threadIdx.x & 15;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row < rows) v = reinterpret_cast<const uint4*>(p.q + (int64_t)(sp.first + row / R) * p.q_stride + (int64_t)(kvh * R + row % R) * kDim)[l];
-    float x[8], top = 0.f;
-    values(unpack8<BF16>(v), x);
-    if (BF16) {                        // (float16 goes in as it is)
+  } else {
+    // the queries, 16 lanes a row, all of a thread's loads under way at once: block of 64 dimensions, row of 128 bytes, piece swizzled by the row
+    constexpr int kWays = kThreads / 16 - 2, kTurns = (kRows + kWays - 1) / kWays;
+    const int way = (threadIdx.x >> 4) - 2, l = threadIdx.x & 15;
+    uint4 v[kTurns];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int k = 0; k < kTurns; ++k) {
+      const int row = i0 + way + k * kWays;
+      v[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (way + k * kWays < kRows && row < rows)
+        v[k] = reinterpret_cast<const uint4*>(p.q + (int64_t)(sp.first + row / R) * p.q_stride + (int64_t)(kvh * R + row % R) * kDim)[l];
     }
-    const float unit = BF16 ? unit_of(top) : 1.f, by = p.sign / unit;
-    v = make_uint4(pack_half(x[0] * by, x[1] * by), pack_half(x[2] * by, x[3] * by), pack_half(x[4] * by, x[5] * by), pack_half(x[6] * by, x[7] * by));
-    if (l == 0) s_row[i] = unit;
-    *reinterpret_cast<uint4*>(smem_q + (i >> 7) * kQBytes + (l >> 3) * kBox + (i & 127) * 128 + (((l & 7) ^ (i & 7)) << 4)) = v;
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+      const int i = way + k * kWays;
+      float x[8], unit = 1.f;
+      values(unpack8<BF16>(v[k]), x);
+      if (BF16) {                      // (float16 goes in as it is)
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        unit = unit_of(top);
+      }
+      if (i >= kRows) break;           // (the same for a warp's two rows)
+      const float by = p.sign / unit;
+      if (l == 0) s_row[i] = unit;
+      *reinterpret_cast<uint4*>(smem_q + (i >> 7) * kQBytes + (l >> 3) * kBox + (i & 127) * 128 + (((l & 7) ^ (i & 7)) << 4)) =
+          make_uint4(pack_half(x[0] * by, x[1] * by), pack_half(x[2] * by, x[3] * by), pack_half(x[4] * by, x[5] * by), pack_half(x[6] * by, x[7] * by));
+    }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the tensor cores read them
   tc_fence_before();
@@ -487,7 +500,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       }
       const float mu = m == -INFINITY ? 0.f : m;
       const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(factor, factor);
-      if (!masked) {
+      auto weights = [&](auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const int left = pos - key0;     // the last key of the half that the row sees
         uint64_t ls[2] = {lsum, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -498,15 +513,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             unpair2(fma2(pair2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), k1, nm2), x0, x1);
             x0 = ex2(x0);
             x1 = ex2(x1);
+            if (EDGE) {
+              x0 = c * 32 + 2 * e <= left ? x0 : 0.f;
+              x1 = c * 32 + 2 * e + 1 <= left ? x1 : 0.f;
+            }
             w[e] = pack_half(x0, x1);
             ls[e & 1] = add2(ls[e & 1], pair2(x0, x1));
           }
           tmem_st16(tS + c * 16, w);
         }
         lsum = add2(ls[0], ls[1]);
+      };
+      if (!masked) {
+        weights(std::false_type());
+      } else if (!s_special) {
+        weights(std::true_type());
       } else {
-        // from tensor memory again, a piece at a time: compact code for the few tiles at the edge, and for sequences with tiles in other units
-        const float by = s_special ? p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].v / s_unit_v : 1.f;      // of the tile's weights in the product
+        // from tensor memory again, a piece at a time: compact code for sequences with tiles in other units
+        const float by = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].v / s_unit_v;      // of the tile's weights in the product
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t v[16], w[8];

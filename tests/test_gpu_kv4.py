@@ -288,6 +288,36 @@ def test_prompt_of_extreme_values(dtype):
     assert torch.isfinite(got).all() and float(got.abs().max()) <= float(v.abs().max()) * (1 + 4 * ref.unit(dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,start", [(5, 300), (400, 0), (90, 700)])
+@torch.no_grad()
+def test_prompt_of_values_far_from_one(n, start, dtype):
+    """Tiles of very large and very small keys and values beside ordinary ones, and queries of any size: what a type holds, the result holds."""
+    from nanoquantization_b200.layers import kv4
+    kv_heads, heads, block, total = 2, 8, 32, n + start
+    kc, vc, table, rows = _cache([total], kv_heads, block, dtype, seed=12)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    big = 4e4 if dtype == torch.float16 else 1e20
+    for c, sizes in ((kc, (1e-4, 1.0, big / 20)), (vc, (big / 20, 1e-5, 1.0))):
+        for h in range(kv_heads):          # runs of 100 keys; the second head's are ten times as small
+            size = torch.tensor(sizes, device=DEV, dtype=torch.float64)[torch.arange(total, device=DEV) // 100 % 3][:, None, None] * 10.0 ** -h
+            x = torch.randn(total, kv_heads, D, generator=g, device=DEV, dtype=torch.float64) * size
+            both = ref.rows_of(c, rows[0], block, dtype)
+            both[:, h] = x[:, h]
+            ref.set_rows(c, rows[0], both, block, dtype)
+    k, v = (ref.rows_of(c, rows[0], block, dtype) for c in (kc, vc))
+    q = torch.randn(n, heads * D, generator=g, device=DEV)
+    q[:, ::2] *= 1e-3
+    q = (q * (1e-3 if dtype == torch.float16 else 1e-9)).to(dtype)
+    scale = 0.5 / float((q.double().view(n, kv_heads, -1, D).norm(dim=-1).amax()) * k.norm(dim=-1).amax())       # scores of one at most
+    cu, pos0 = torch.tensor([0, n], dtype=torch.int32, device=DEV), torch.tensor([start], dtype=torch.int32, device=DEV)
+    got = kv4.prompt_attention(q, heads, kc, vc, table, cu, pos0, [n], [start], scale=scale * 8)
+    want = ref.attend(q.double().view(n, heads, D), k, v, start, scale * 8).flatten(1)
+    _close(got, want, dtype)
+    small = kv4.prompt_attention(q, heads, kc, vc, table, cu, pos0, [n], [start], scale=-scale)
+    _close(small, ref.attend(q.double().view(n, heads, D), k, v, start, -scale).flatten(1), dtype)
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("dtype", TYPES)
 @torch.no_grad()
