@@ -67,7 +67,7 @@ struct Params {
   TileInfo* info;        // [tile][kv head]
   float* shares;
   int heads, tokens, batch, parts, max_len, max_ctx, total;     // total: tiles that there is room for
-  float factor;          // scale log2 e, not negative
+  float factor;          // scale log2 e, above 0 (a masked score stays minus infinity)
   float sign;            // of the scale: the queries take it
   int* status;
 };
@@ -228,9 +228,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     mbar_fence_init();
   }
   if (warp == 1) { tmem_alloc(smem_u32(&s_tmem), kTmemCols); tmem_relinquish(); }
+  // A ring stage's first tiles are under way while the queries come in.
+  const auto tile_src = [&](int j) { return p.tiles + ((int64_t)(s_before + first + j) * p.cache.kv_heads + kvh) * (2 * (int64_t)kTileBytes); };
+  const auto copy = [&](uint32_t dst, const uint8_t* src, uint64_t* bar) {
+    mbar_expect_tx(smem_u32(bar), kTileBytes);
+    bulk_load(dst, src, kTileBytes, smem_u32(bar));
+  };
   if (warp == 0) {
     const int before = tiles_before(p, b);
     if (lane == 0) s_before = before;
+    __syncwarp();
+    if (before + first + nmax <= p.total && elect_one()) {
+      for (int j = 0; j < min(nmax, 2); ++j) {
+        copy(smem + kOffK + j * kTileBytes, tile_src(j), &bar_kfull[j]);
+        copy(smem + kOffV + j * kTileBytes, tile_src(j) + kTileBytes, &bar_vfull[j]);
+      }
+    }
   } else {
     // the queries, 16 lanes a row, all of a thread's loads under way at once: block of 64 dimensions, row of 128 bytes, piece swizzled by the row
     constexpr int kWays = kThreads / 16 - 2, kTurns = (kRows + kWays - 1) / kWays;
@@ -278,23 +291,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   if (warp == 0) {
     // --------------------------------------------------------------- copies
     const bool el = elect_one();
-    int issued = 0;
-    for (int j = 0; j < n_tiles; ++j, ++issued) {
+    int issued = min(n_tiles, 2);
+    for (int j = 2; j < n_tiles; ++j, ++issued) {
       const int s = j & 1;
-      const uint8_t* src = p.tiles + ((int64_t)(tile0 + j) * p.cache.kv_heads + kvh) * (2 * (int64_t)kTileBytes);
-      if (j >= 2 && !wait_bar_warp(&bar_kfree[s], ((j >> 1) - 1) & 1, s_abort, p.status)) break;
-      if (el) {
-        mbar_expect_tx(smem_u32(&bar_kfull[s]), kTileBytes);
-        bulk_load(smem + kOffK + s * kTileBytes, src, kTileBytes, smem_u32(&bar_kfull[s]));
-      }
-      if (j >= 2 && !wait_bar_warp(&bar_vfree[s], ((j >> 1) - 1) & 1, s_abort, p.status)) {
+      if (!wait_bar_warp(&bar_kfree[s], ((j >> 1) - 1) & 1, s_abort, p.status)) break;
+      if (el) copy(smem + kOffK + s * kTileBytes, tile_src(j), &bar_kfull[s]);
+      if (!wait_bar_warp(&bar_vfree[s], ((j >> 1) - 1) & 1, s_abort, p.status)) {
         mbar_wait(smem_u32(&bar_kfull[s]), (j >> 1) & 1);
         break;
       }
-      if (el) {
-        mbar_expect_tx(smem_u32(&bar_vfull[s]), kTileBytes);
-        bulk_load(smem + kOffV + s * kTileBytes, src + kTileBytes, kTileBytes, smem_u32(&bar_vfull[s]));
-      }
+      if (el) copy(smem + kOffV + s * kTileBytes, tile_src(j) + kTileBytes, &bar_vfull[s]);
     }
     // do not leave while a copy may still be landing
     for (int j = issued > 2 ? issued - 2 : 0; j < issued; ++j) {
@@ -443,31 +449,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld32(tS + c * 32, r[c]);
       tc_wait_ld();
+      // what the row does not see: scores below all others
+      const int left = pos - key0;
+      auto mask = [&](uint32_t (&v)[32], int from) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = from + e <= left ? v[e] : 0xFF800000u;
+      };
       float mx = -INFINITY;  // where it is asked for, the largest score
-      float ab = 0.f;        // the largest magnitude
-      if (!masked) {
+      bool look = joint || masked;
+      if (masked) {
+        mask(r[0], 0);
+        mask(r[1], 32);
+      } else if (!joint) {   // a half finds out from the largest magnitude that nothing moves
         float hi[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3_abs(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-        ab = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
+        look = !__all_sync(0xFFFFFFFFu, fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])) * factor <= m + kLag);
       }
       const float lag = m + kLag;
-      if (joint || masked || !__all_sync(0xFFFFFFFFu, ab * factor <= lag)) {
-        if (!masked) {
-          float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (look) {
+        float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-          mx = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
-        } else {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) mx = key0 + c * 32 + e <= pos ? fmaxf(mx, __uint_as_float(r[c][e])) : mx;
-        }
+          for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+        mx = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
         if (joint) {
           float mo;
           if (!(ok = exchange(mx, mo))) break;
@@ -497,12 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         tc_wait_st();
         tmem_ld32(tS, r[0]);      // the scores again
         tc_wait_ld();
+        if (masked) mask(r[0], 0);
       }
       const float mu = m == -INFINITY ? 0.f : m;
       const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(factor, factor);
-      auto weights = [&](auto edge) {
-        constexpr bool EDGE = decltype(edge)::value;
-        const int left = pos - key0;     // the last key of the half that the row sees
+      if (!masked || !s_special) {
         uint64_t ls[2] = {lsum, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -513,21 +520,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
             unpair2(fma2(pair2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), k1, nm2), x0, x1);
             x0 = ex2(x0);
             x1 = ex2(x1);
-            if (EDGE) {
-              x0 = c * 32 + 2 * e <= left ? x0 : 0.f;
-              x1 = c * 32 + 2 * e + 1 <= left ? x1 : 0.f;
-            }
             w[e] = pack_half(x0, x1);
             ls[e & 1] = add2(ls[e & 1], pair2(x0, x1));
           }
           tmem_st16(tS + c * 16, w);
         }
         lsum = add2(ls[0], ls[1]);
-      };
-      if (!masked) {
-        weights(std::false_type());
-      } else if (!s_special) {
-        weights(std::true_type());
       } else {
         // from tensor memory again, a piece at a time: compact code for sequences with tiles in other units
         const float by = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].v / s_unit_v;      // of the tile's weights in the product
@@ -549,10 +547,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       }
       done();
     }
+    // Rows go out through shared memory (the queries' place, which no product reads any more), so that a store's lanes write to four lines and
+    // not to 32: a warp stages its 32 rows x 128 bytes, piece c of row r at c ^ r mod 8.
     const int R = p.heads / p.cache.kv_heads, at = min(i, span_of(p, blockIdx.z).n * R - 1);      // (again, rather than in registers until here)
-    const int64_t out_row = (int64_t)(p.cu[blockIdx.z] + at / R) * p.heads + blockIdx.y * R + at % R;
-    const bool mine = at == i;
-    float* share = p.shares + (out_row * p.parts + blockIdx.x % p.parts) * kShare + half * 64;
+    const int out_row = at == i ? (p.cu[blockIdx.z] + at / R) * p.heads + (int)blockIdx.y * R + at % R : -1;
+    const bool shares = p.parts > 1;
+    uint8_t* stage = smem_q + q * kQBytes + (half * 4 + quarter) * 4096;
+    const auto put = [&](int c, uint4 v) { *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = v; };
+    const auto write = [&](uint8_t* base, int64_t row_bytes, int64_t offset) {
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = k * 4 + (lane >> 3), to = __shfl_sync(0xFFFFFFFFu, out_row, r);
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        if (to >= 0) *reinterpret_cast<uint4*>(base + to * row_bytes + offset + (lane & 7) * 16) = v;
+      }
+      __syncwarp();
+    };
+    float* const share0 = p.shares + (blockIdx.x % p.parts) * kShare;
+    const int64_t share_row = (int64_t)p.parts * kShare * sizeof(float);
     if (ok && nq[q] > 0) {
       ok = (half == 1 || catch_up(nq[q])) && wait_bar_warp(&bar_o[q], 0, s_abort, p.status);
       float l = 0.f;
@@ -567,42 +580,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         tc_fence_after();
         // dimensions 64 half ..: NaN where a value that the row sees is none
         const float poison = s_bad[half] <= pos ? __int_as_float(0x7FC00000) : 0.f;
-        const float f = p.parts > 1 ? s_unit_v : s_unit_v / l;
-        uint16_t* dst = p.out + out_row * kDim + half * 64;
+        const float f = shares ? s_unit_v : s_unit_v / l;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t r[32];
           tmem_ld32(tO + half * 64 + c * 32, r);
           tc_wait_ld();
-          if (mine) {
-            if (p.parts > 1) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(share + c * 32 + e * 4) =
-                    make_float4(fmaf(__uint_as_float(r[4 * e]), f, poison), fmaf(__uint_as_float(r[4 * e + 1]), f, poison),
-                                fmaf(__uint_as_float(r[4 * e + 2]), f, poison), fmaf(__uint_as_float(r[4 * e + 3]), f, poison));
-            } else {
+          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), f, poison));
+          if (shares) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint4 v;
-                v.x = pack16<BF16>(fmaf(__uint_as_float(r[8 * e]), f, poison), fmaf(__uint_as_float(r[8 * e + 1]), f, poison));
-                v.y = pack16<BF16>(fmaf(__uint_as_float(r[8 * e + 2]), f, poison), fmaf(__uint_as_float(r[8 * e + 3]), f, poison));
-                v.z = pack16<BF16>(fmaf(__uint_as_float(r[8 * e + 4]), f, poison), fmaf(__uint_as_float(r[8 * e + 5]), f, poison));
-                v.w = pack16<BF16>(fmaf(__uint_as_float(r[8 * e + 6]), f, poison), fmaf(__uint_as_float(r[8 * e + 7]), f, poison));
-                *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = v;
-              }
-            }
+            for (int e = 0; e < 8; ++e) put(e, make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]));
+            write((uint8_t*)share0, share_row, half * 256 + c * 128);
+          } else {
+            const auto two = [&](int e) { return pack16<BF16>(__uint_as_float(r[e]), __uint_as_float(r[e + 1])); };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) put(4 * c + e, make_uint4(two(8 * e), two(8 * e + 2), two(8 * e + 4), two(8 * e + 6)));
           }
-          __syncwarp();
         }
-        if (p.parts > 1 && mine && half == 0) { share[kDim] = m; share[kDim + 1] = l; }
+        if (!shares) write((uint8_t*)p.out, kDim * 2, half * 128);
+        if (shares && out_row >= 0 && half == 0) { share0[(int64_t)out_row * p.parts * kShare + kDim] = m; share0[(int64_t)out_row * p.parts * kShare + kDim + 1] = l; }
         tc_fence_before();
       }
-    } else if (nq[q] == 0 && p.parts > 1 && mine) {      // no keys of this part, or none that could be read
-      for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(share + e * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (half == 0) { share[kDim] = -INFINITY; share[kDim + 1] = 0.f; }
-    } else if (nq[q] == 0 && mine) {
-      for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(p.out + out_row * kDim + half * 64 + e * 8) = make_uint4(0u, 0u, 0u, 0u);
+    } else if (nq[q] == 0) {      // no keys of this part, or none that could be read
+#pragma unroll
+      for (int e = 0; e < 8; ++e) put(e, make_uint4(0u, 0u, 0u, 0u));
+      if (shares) {
+        write((uint8_t*)share0, share_row, half * 256);
+        write((uint8_t*)share0, share_row, half * 256 + 128);
+        if (out_row >= 0 && half == 0) { share0[(int64_t)out_row * p.parts * kShare + kDim] = -INFINITY; share0[(int64_t)out_row * p.parts * kShare + kDim + 1] = 0.f; }
+      } else {
+        write((uint8_t*)p.out, kDim * 2, half * 128);
+      }
     }
   }
   // all roles meet here, also after a give-up, so that tensor memory is always released
@@ -640,7 +649,7 @@ int prompt_umma(const uint16_t* q, int64_t q_stride, const nqb200_kv4* cache, co
   p.tiles = (uint8_t*)scratch; p.info = (TileInfo*)(p.tiles + tile_bytes(tiles, hk)); p.shares = (float*)((uint8_t*)p.info + info_bytes(tiles, hk));
   p.heads = (int)heads; p.tokens = (int)tokens; p.batch = (int)batch; p.max_len = (int)max_len; p.max_ctx = (int)max_ctx; p.total = (int)tiles;
   p.parts = parts_of(batch, max_len, max_ctx, heads, hk);
-  p.factor = fabsf(scale) * kLog2e; p.sign = scale < 0.f ? -1.f : 1.f; p.status = status;
+  p.factor = fmaxf(fabsf(scale) * kLog2e, 1e-37f); p.sign = scale < 0.f ? -1.f : 1.f; p.status = status;
   const bool bf16 = dtype == NQB200_BF16;
   const dim3 expand((unsigned)((max_ctx + kTileKeys - 1) / kTileKeys), (unsigned)hk, (unsigned)batch);
   int rc = launch_overlapped(bf16 ? kv4_expand_kernel<true> : kv4_expand_kernel<false>, expand, dim3(512), 0, st, p);
