@@ -261,6 +261,10 @@ int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, const nqb200_kv
 size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads,
                                        int64_t kv_heads);
 
+/* Which kernels that call takes ("rows", "tiles_tcgen05"); for logs and tests. */
+const char* nqb200_kv4_prompt_kernel_name(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads,
+                                          int64_t kv_heads);
+
 /* Copies of pages, or of any rows of equal size: for every pool p and pair i, row_bytes[p] bytes from row sources[i] to row
  * targets[i] of pools[p], all on one device.  The numbers are read during the call (host memory).  The same target twice, or a
  * target that is also a source, is refused, as is a row outside [0, rows). */

@@ -65,6 +65,7 @@ SIGNATURES = {
     "nqb200_kv4_decode_scratch_bytes": (_sz, [_i64] * 5),
     "nqb200_kv4_prompt_attention": (_int, [_vp, _i64, _kv4, _vp, _i64, _vp, _vp, _vp] + [_i64] * 6 + [ctypes.c_float, _int, _vp, _sz, _vp, _vp]),
     "nqb200_kv4_prompt_scratch_bytes": (_sz, [_i64] * 7),
+    "nqb200_kv4_prompt_kernel_name": (ctypes.c_char_p, [_i64] * 7),
     "nqb200_copy_pages": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "nqb200_silu_mul": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "nqb200_comm_alloc": (_int, [ctypes.POINTER(_vp), _sz]),

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   const int first_pos = DECODE ? 0 : a.pos0[b];
   // column c: row group * 8 + c of the sequence's (token, head of the group) rows
   const auto token_of = [&](int c) { return (group * kCols + c) / R; };
-  int keys = DECODE ? a.ctx[b] : first_pos + token_of(cols - 1) + 1;
+  int keys = DECODE ? a.ctx[b] : (int)min((int64_t)first_pos + token_of(cols - 1) + 1, (int64_t)INT32_MAX);
   const int64_t room = (int64_t)a.width * a.cache.block;
   if (keys > room || (!DECODE && (first_pos < 0 || n_tokens > a.max_len))) {
     if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
@@ -699,11 +699,23 @@ extern "C" int nqb200_kv4_decode_attention(const void* qkv, int64_t row_stride, 
   return launch<true>(a, batch, batch, table_width * cache->block_size, dtype, (cudaStream_t)stream);
 }
 
+// Few rows or many; what does not fit into the grid of the way for few goes the other way.
+static bool prompt_goes_umma(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
+  return kv_heads * groups_of(max_len, heads, kv_heads) > 65535 || kv4::prompt_umma_faster(batch, T, max_len, max_ctx, tiles, heads, kv_heads);
+}
+
 extern "C" size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads, int64_t kv_heads) {
-  if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || batch > 65535 || T <= 0 || max_len <= 0 || max_ctx < max_len) return 0;
-  if (kv4::prompt_umma_supports(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads))
+  if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || batch > 65535 || T <= 0 || max_len <= 0 || max_len > T || max_ctx < max_len || max_ctx > INT32_MAX - 256 || tiles <= 0 ||
+      tiles > INT32_MAX / 2)
+    return 0;
+  if (prompt_goes_umma(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads))
     return kv4::prompt_umma_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads);
   return scratch_bytes_of(batch, T, max_len, max_ctx, num_q_heads, kv_heads);
+}
+
+extern "C" const char* nqb200_kv4_prompt_kernel_name(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads, int64_t kv_heads) {
+  if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || T <= 0 || max_len <= 0 || max_ctx < max_len || tiles <= 0) return "invalid";
+  return prompt_goes_umma(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads) ? "tiles_tcgen05" : "rows";
 }
 
 extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, const nqb200_kv4* cache, const int32_t* table, int64_t table_width,
@@ -711,13 +723,13 @@ extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, cons
                                            int64_t tiles, int64_t num_q_heads, float scale, int dtype, void* scratch, size_t scratch_bytes, int* status, void* stream) {
   const int rc = check_heads(cache, num_q_heads, table_width, dtype);
   if (rc != NQB200_OK) return rc;
-  if (batch < 0 || batch > 65535 || T < 0 || T > INT32_MAX / num_q_heads || max_len < 0 || (T > 0 && max_len > T) || max_ctx < max_len || max_ctx > INT32_MAX || tiles < 0 ||
+  if (batch < 0 || batch > 65535 || T < 0 || T > INT32_MAX / num_q_heads || max_len < 0 || (T > 0 && max_len > T) || max_ctx < max_len || max_ctx > INT32_MAX - 256 || tiles < 0 || tiles > INT32_MAX / 2 ||
       q_stride < num_q_heads * kv4::kDim || q_stride % 8 != 0)
     return NQB200_ERR_BAD_SHAPE;
   if (batch == 0 || T == 0) return NQB200_OK;
   const int64_t groups = groups_of(max_len, num_q_heads, cache->kv_heads);
-  const bool umma = kv4::prompt_umma_supports(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);
-  if (max_len == 0 || (!umma && cache->kv_heads * groups > 65535)) return NQB200_ERR_BAD_SHAPE;
+  if (max_len == 0 || tiles == 0) return NQB200_ERR_BAD_SHAPE;
+  const bool umma = prompt_goes_umma(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);
   if (!q || !table || !cu || !pos0 || !out) return NQB200_ERR_NULL_POINTER;
   if (!aligned16(q) || !aligned16(out)) return NQB200_ERR_MISALIGNED;
   const size_t need = nqb200_kv4_prompt_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, cache->kv_heads);

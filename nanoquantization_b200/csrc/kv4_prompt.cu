@@ -80,7 +80,7 @@ __device__ __forceinline__ Span span_of(const Params& p, int b) {
   s.n = p.cu[b + 1] - s.first;
   s.pos0 = p.pos0[b];
   if (s.first < 0 || s.n < 0 || s.n > p.max_len || s.n > p.tokens - s.first || s.pos0 < 0) s.n = 0;      // reported by expand
-  s.keys = s.n > 0 ? (int)min((int64_t)min(s.pos0 + s.n, p.max_ctx), p.width * p.cache.block) : 0;
+  s.keys = s.n > 0 ? (int)min(min((int64_t)s.pos0 + s.n, (int64_t)p.max_ctx), p.width * p.cache.block) : 0;
   return s;
 }
 // Tiles of the sequences before b; by all threads of a warp.
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(512) kv4_expand_kernel(const __grid_constant__
   const Span s = span_of(p, b);
   if (tile == 0 && h == 0 && threadIdx.x == 0) {
     const int n = p.cu[b + 1] - p.cu[b];
-    if (s.n != n || (n > 0 && s.keys != s.pos0 + n)) report(p.status, NQB200_ERR_BAD_INDEX);
+    if (s.n != n || (n > 0 && s.keys != (int64_t)s.pos0 + n)) report(p.status, NQB200_ERR_BAD_INDEX);
   }
   const int key0 = tile * kTileKeys;
   if (key0 >= s.keys) return;
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   const int i0 = (int)(gridDim.x / p.parts - 1 - blockIdx.x / p.parts) * kRows;     // long rows first
   if (i0 >= rows) return;
   // key tiles of this CTA, from `first` on, for each query tile
-  const auto pos_of = [&](int row) { return sp.pos0 + min(row, rows - 1) / R; };
+  const auto pos_of = [&](int row) { return (int)min((int64_t)sp.pos0 + min(row, rows - 1) / R, (int64_t)INT32_MAX); };
   const auto tiles_of = [&](int q) { return i0 + q * 128 < rows ? min(pos_of(i0 + q * 128 + 127), sp.keys - 1) / kTileKeys + 1 : 0; };
   const int all = max(tiles_of(0), tiles_of(1)), per = (all + p.parts - 1) / p.parts, first = part * per;
   int nq[2];
@@ -633,8 +633,19 @@ int parts_of(int64_t batch, int64_t max_len, int64_t max_ctx, int64_t heads, int
 
 }  // namespace
 
-bool prompt_umma_supports(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
-  return max_len * (heads / kv_heads) >= kUmmaRows && tiles > 0 && tiles <= INT32_MAX / 2 && max_ctx <= INT32_MAX - 256;
+// Which of the two ways a call takes: the one that is expected to end first, in us, by what 68 calls of either took (16 to 512 tokens of 1 to 32
+// sequences behind 0 to 16000, 2 to 8 query heads per key/value head, 1 and 8 of those; a wrong choice costs 2 us, and up to 10 for
+// long drafts of one key/value head).  Few rows: a CTA per 8 of them goes over the keys.  Many: the pages taken apart, then tiles of
+// 256 rows x 128 keys one after the other.  64 tokens of 32 heads over 8: 7.2 and 16.2 us alone, 27 and 31 behind 2000, 148 and 60 behind 16000.
+bool prompt_umma_faster(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
+  const double rows = (double)tokens * (heads / kv_heads), mean_keys = fmax(1.0, 128.0 * tiles / batch - 0.5 * tokens / batch);
+  const double units = (rows / 8 + 0.5 * batch) * kv_heads, few = 5.0 + units * 0.010 + units * mean_keys / 30000;
+  const int64_t key_tiles = (max_ctx + kTileKeys - 1) / kTileKeys, parts = parts_of(batch, max_len, max_ctx, heads, kv_heads);
+  const double ctas = fmax(rows / kRows, (double)batch) * kv_heads * parts, turns = ctas > kNumSMs ? ctas / kNumSMs : 1.0;
+  const bool fresh = max_ctx < 2 * max_len;      // half of the tiles lie behind the mask
+  const double many = 12.0 + (max_len * (heads / kv_heads) > 128 ? 2.8 : 0.0) + 0.017 * tiles * kv_heads +
+                      2.2 * turns * ((key_tiles + parts - 1) / parts) * (fresh && key_tiles > 2 ? 0.55 : 1.0) + (parts > 1 ? 3.0 : 0.0);
+  return many < few;
 }
 size_t prompt_umma_scratch_bytes(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
   const int parts = parts_of(batch, max_len, max_ctx, heads, kv_heads);

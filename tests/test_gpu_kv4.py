@@ -244,6 +244,97 @@ def test_prompt(lens, starts, kv_heads, heads, block, dtype):
         o += n
 
 
+# what the tensor cores' tiles of 256 rows and 128 keys take: ragged prompts, groups that do not divide a tile, keys dealt to several CTAs, edges
+MANY = [((300,) * 8, (0,) * 8, 8, 32, 256), ((257, 40, 700, 1), (0, 1500, 127, 9), 8, 64, 48), ((64,), (16000,), 2, 32, 256), ((1030,), (0,), 4, 12, 32), ((90, 500), (5000, 3), 4, 28, 64),
+        ((520, 130), (0, 0), 8, 40, 16), ((256, 512), (0, 128), 16, 64, 128), ((1500,), (513,), 8, 8, 256)]
+
+
+def _kernel(lens, starts, heads, kv_heads):
+    from nanoquantization_b200 import _lib
+    ends = [n + s for n, s in zip(lens, starts) if n]
+    return _lib.load().nqb200_kv4_prompt_kernel_name(len(lens), sum(lens), max(lens), max(ends), sum(-(-e // 128) for e in ends), heads, kv_heads)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,starts,kv_heads,heads,block", MANY, ids=str)
+@torch.no_grad()
+def test_prompt_of_many_rows(lens, starts, kv_heads, heads, block, dtype):
+    from nanoquantization_b200.layers import kv4
+    assert _kernel(lens, starts, heads, kv_heads) == b"tiles_tcgen05"
+    ends = [n + s for n, s in zip(lens, starts)]
+    kc, vc, table, rows = _cache(ends, kv_heads, block, dtype, seed=5, width=2)
+    T = sum(lens)
+    q = torch.randn(T, heads * D, generator=torch.Generator(device=DEV).manual_seed(6), device=DEV).to(dtype)
+    cu = torch.tensor([0, *lens], device=DEV).cumsum(0).int()
+    got = kv4.prompt_attention(q, heads, kc, vc, table, cu, torch.tensor(starts, dtype=torch.int32, device=DEV), lens, starts)
+    again = kv4.prompt_attention(q, heads, kc, vc, table, cu, torch.tensor(starts, dtype=torch.int32, device=DEV), lens, starts)
+    assert torch.equal(got, again)
+    R, o = heads // kv_heads, 0
+    for b, n in enumerate(lens):
+        k, v = (ref.rows_of(c, rows[b], block, dtype) for c in (kc, vc))
+        x = q[o:o + n].double().view(n, heads, D)
+        seen = torch.arange(ends[b], device=DEV) <= starts[b] + torch.arange(n, device=DEV)[:, None]
+        for h in {0, R - 1, heads // 2, heads - 1}:
+            w = torch.softmax((x[:, h] @ k[:, h // R].T * D ** -0.5).masked_fill(~seen, float("-inf")), -1)
+            want, mine = w @ v[:, h // R], got[o:o + n].view(n, heads, D)[:, h]
+            _close(mine, want, dtype)
+            worst = (mine.double() - want).norm(dim=-1) / want.norm(dim=-1)
+            assert float(worst.max()) <= 4 * ref.unit(dtype), (b, h, int(worst.argmax()))
+        o += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@torch.no_grad()
+def test_prompt_of_many_rows_with_values_that_are_not_finite(dtype):
+    """As below, for the tiles: also where the keys are dealt to several CTAs."""
+    from nanoquantization_b200.layers import kv4
+    for n, start, kv_heads, heads in ((700, 50, 8, 32), (64, 9000, 2, 32)):
+        assert _kernel([n], [start], heads, kv_heads) == b"tiles_tcgen05"
+        block, R = 64, heads // kv_heads
+        kc, vc, table, rows = _cache([start + n], kv_heads, block, dtype, seed=8)
+        q = torch.randn(n, heads * D, device=DEV).to(dtype)
+        cu, pos0 = torch.tensor([0, n], dtype=torch.int32, device=DEV), torch.tensor([start], dtype=torch.int32, device=DEV)
+        run = lambda: kv4.prompt_attention(q, heads, kc, vc, table, cu, pos0, [n], [start])  # noqa: E731
+        want, i = run(), n // 2
+        r = rows[0][start + i]
+        vc[..., block * 64:].unflatten(-1, (block, 8))[r // block, 1, r % block, 4:6] = 255             # the second group's scale of head 1
+        got = run()
+        nan = torch.zeros(n, kv_heads, R, 2, 64, dtype=torch.bool, device=DEV)
+        nan[i:, 1, :, 1] = True
+        nan = nan.view(n, -1)
+        assert got[nan].isnan().all() and torch.equal(got[~nan], want[~nan])
+        kc[..., block * 64:].unflatten(-1, (block, 8))[r // block, 0, r % block, 2:4] = 255             # the first group's offset of head 0
+        got = run().view(n, kv_heads, -1)
+        assert got[i:, 0].isnan().all() and torch.equal(got[:i], want.view(n, kv_heads, -1)[:i])
+
+
+@torch.no_grad()
+def test_prompt_bad_pages_of_many_rows():
+    from nanoquantization_b200 import _lib
+    from nanoquantization_b200.layers import kv4
+    lens, starts, kv_heads, heads, block, dtype = [300, 300], [0, 400], 8, 32, 32, torch.bfloat16
+    assert _kernel(lens, starts, heads, kv_heads) == b"tiles_tcgen05"
+    kc, vc, table, rows = _cache([300, 700], kv_heads, block, dtype, seed=2)
+    q = torch.randn(600, heads * D, device=DEV).to(dtype)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    run = lambda t=table, cu=i32(0, 300, 600), pos0=i32(*starts): kv4.prompt_attention(q, heads, kc, vc, t, cu, pos0, lens, starts)  # noqa: E731
+    good = run()
+    _lib.check_cache_status()
+    for at, page in ((3, -1), (0, len(kc)), (21, 1 << 30)):
+        t = table.clone()
+        t[1, at] = page
+        got = run(t)
+        assert torch.equal(got[:300], good[:300])
+        with pytest.raises(RuntimeError, match="outside its buffer"):
+            _lib.check_cache_status()
+    # numbers on the device that are not those of the host: more keys, more tokens, tokens that are none of q's
+    for kw in ({"pos0": i32(0, 30000)}, {"pos0": i32(0, -3)}, {"cu": i32(0, 300, 700)}, {"cu": i32(0, 300, 100)}, {"cu": i32(0, 300, 1 << 30)}):
+        got = run(**kw)
+        assert torch.equal(got[:300], good[:300])
+        with pytest.raises(RuntimeError, match="outside its buffer"):
+            _lib.check_cache_status()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [3, 70, 400])
 @torch.no_grad()

@@ -57,6 +57,16 @@ def test_refusals_of_the_attention():
     assert prompt(q=None) == prompt(table=None) == prompt(cu=None) == prompt(out=None) == 4 and prompt(q=P + 8) == prompt(out=P + 8) == 3
 
 
+def test_which_way_a_prompt_takes():
+    name = _lib.load().nqb200_kv4_prompt_kernel_name
+    assert name(1, 0, 1, 1, 1, 4, 2) == name(0, 1, 1, 1, 1, 4, 2) == name(1, 1, 1, 1, 1, 4, 3) == name(1, 2, 2, 1, 1, 4, 2) == b"invalid"
+    for heads in (16, 32, 64):
+        assert name(1, 16, 16, 16, 1, heads, 8) == name(4, 20, 5, 3006, 96, heads, 8) == b"rows"
+        assert name(1, 8000, 8000, 8000, 63, heads, 8) == name(1, 500, 500, 12500, 98, heads, 8) == b"tiles_tcgen05"
+    # 65536 columns of eight and more do not fit into the grid of the way for few rows
+    assert name(1, 1 << 20, 1 << 20, 1 << 20, 1 << 13, 8, 8) == b"tiles_tcgen05"
+
+
 def test_refusals_of_the_copies():
     lib = _lib.load()
 
