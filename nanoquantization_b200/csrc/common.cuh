@@ -53,6 +53,19 @@ static inline void prefer_loads() {
   done.fetch_or(bit, std::memory_order_relaxed);
 }
 
+// Lets a kernel take `bytes` of dynamic shared memory, once per kernel and device.
+template <auto Kernel>
+static inline bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) { cudaGetLastError(); return false; }
+  const uint64_t bit = dev < kMaxDevices ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) { cudaGetLastError(); return false; }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 // How the split-K decode kernel tiles a problem; the same plan sizes the workspace.
 struct DecodePlan {
   int mt;        // 8-token tiles per CTA (1 or 2)

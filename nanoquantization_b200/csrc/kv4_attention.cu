@@ -621,9 +621,9 @@ Split split(int64_t units, int64_t keys) {
 int groups_of(int64_t tokens, int64_t heads, int64_t kv_heads) { return (int)((tokens * (heads / kv_heads) + kCols - 1) / kCols); }
 
 template <bool BF16, bool DECODE, int STAGES> int launch_stages(const Args& a, int csize, int64_t batch, cudaStream_t st) {
-  const auto kernel = kv4_rows_kernel<BF16, DECODE, STAGES>;
+  constexpr auto kernel = kv4_rows_kernel<BF16, DECODE, STAGES>;
   constexpr int smem = smem_bytes(STAGES);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) { cudaGetLastError(); return NQB200_ERR_LAUNCH; }
+  if (!allow_smem<kernel>(smem)) return NQB200_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(csize * a.parts), (unsigned)(a.cache.kv_heads * a.groups), (unsigned)batch);
   cfg.blockDim = dim3(kThreads);

@@ -667,7 +667,7 @@ int prompt_umma(const uint16_t* q, int64_t q_stride, const nqb200_kv4* cache, co
   if (rc != NQB200_OK) return rc;
   const auto kernel = bf16 ? kv4_prompt_kernel<true> : kv4_prompt_kernel<false>;
   constexpr int smem = 2 * 128 * kDim * 2 + 4 * (int)kTileBytes + 1024;       // one CTA per SM, because a CTA takes all of its tensor memory
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) { cudaGetLastError(); return NQB200_ERR_LAUNCH; }
+  if (!(bf16 ? allow_smem<kv4_prompt_kernel<true>>(smem) : allow_smem<kv4_prompt_kernel<false>>(smem))) return NQB200_ERR_LAUNCH;
   const dim3 grid((unsigned)((max_len * (heads / hk) + kRows - 1) / kRows * p.parts), (unsigned)hk, (unsigned)batch);
   rc = launch_overlapped(kernel, grid, dim3(kThreads), smem, st, p);
   if (rc != NQB200_OK || p.parts == 1) return rc;

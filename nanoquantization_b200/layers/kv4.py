@@ -94,8 +94,7 @@ def load(k_cache: torch.Tensor, v_cache: torch.Tensor, rows: torch.Tensor, dtype
     cache, code, n = _cache(k_cache, v_cache), _lib.dtype_code(dtype), rows.numel()
     _ints("rows", rows, torch.int64, (n,))
     with _lib.on_device(dev) as stream:
-        shape = (n, cache.kv_heads, DIM)
-        k, v = k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+        k, v = k_cache.new_empty((2, n, cache.kv_heads, DIM), dtype=dtype).unbind()
         status = _lib.load().nqb200_kv4_load(cache, rows.data_ptr(), k.data_ptr(), v.data_ptr(), n, code, _lib.cache_status(dev), stream)
     _lib.check(status)
     return k, v

@@ -582,3 +582,17 @@ def test_copies_of_pools_that_start_anywhere():
         want = base.clone()
         want[at:at + 5 * nbytes].view(5, nbytes)[[3, 1]] = base[at:at + nbytes]
         assert torch.equal(mine, want)
+
+
+@torch.no_grad()
+def test_copies_of_pools_that_do_not_fit():
+    from nanoquantization_b200.layers.pages import copy_pages
+    a = torch.zeros(4, 6, device=DEV)
+    for pools in ([a, torch.zeros(5, 6, device=DEV)], [a, a.T], [a, torch.zeros(4, 6)], [a, torch.zeros((), device=DEV)], [torch.zeros((), device=DEV)], [torch.zeros(0, 6, device=DEV)]):
+        with pytest.raises((ValueError, RuntimeError), match="pools must be|CUDA tensors only"):
+            copy_pages(pools, [0], [1])
+    for src, dst in (([0], [4]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 2], [2, 3]), ([1 << 33], [0])):
+        with pytest.raises(ValueError, match="every target once"):
+            copy_pages([a], src, dst)
+    with pytest.raises(RuntimeError, match="bad shape"):
+        copy_pages([torch.zeros(4, 0, device=DEV)], [0], [1])
