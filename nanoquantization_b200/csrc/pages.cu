@@ -61,8 +61,8 @@ extern "C" int nqb200_copy_pages(void* const* pools, const int64_t* row_bytes, i
   if (n_pairs > rows) return NQB200_ERR_BAD_INDEX;         // some target comes twice
   int64_t most = 0;
   for (int64_t p = 0; p < n_pools; ++p) {
-    if (!pools[p]) return NQB200_ERR_NULL_POINTER;
     if (row_bytes[p] <= 0) return NQB200_ERR_BAD_SHAPE;
+    if (!pools[p]) return NQB200_ERR_NULL_POINTER;
     most = std::max(most, row_bytes[p]);
   }
   for (int64_t i = 0; i < n_pairs; ++i)
