@@ -309,6 +309,19 @@ def test_prompt_of_many_rows_with_values_that_are_not_finite(dtype):
 
 
 @torch.no_grad()
+def test_prompts_that_are_taken_in_several_goes(monkeypatch):
+    from nanoquantization_b200.layers import kv4
+    lens, starts, kv_heads, heads, block, dtype = [200, 1, 0, 400, 90, 30, 700], [0, 900, 7, 100, 0, 0, 300], 4, 16, 32, torch.bfloat16
+    kc, vc, table, rows = _cache([n + s if n else 0 for n, s in zip(lens, starts)], kv_heads, block, dtype, seed=4)
+    q = torch.randn(sum(lens), heads * D, device=DEV).to(dtype)
+    cu, pos0 = torch.tensor([0, *lens], device=DEV).cumsum(0).int(), torch.tensor(starts, dtype=torch.int32, device=DEV)
+    want = kv4.prompt_attention(q, heads, kc, vc, table, cu, pos0, lens, starts)
+    for tiles in (1, 5, 9, 12):
+        monkeypatch.setattr(kv4, "MOST_SCRATCH", tiles * 128 * 512 * kv_heads)
+        _close(kv4.prompt_attention(q, heads, kc, vc, table, cu, pos0, lens, starts), want.double(), dtype)
+
+
+@torch.no_grad()
 def test_prompt_bad_pages_of_many_rows():
     from nanoquantization_b200 import _lib
     from nanoquantization_b200.layers import kv4
