@@ -85,6 +85,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
 // Nibbles I and I + 4 of a word, as pairs of float16: 1024 + n for even I, 1024 + 16 n for odd I.  `magic` is a pair of 1024 in a register:
 // with two immediate operands it would be two instructions.
 struct Lifted { uint32_t v[4]; };
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   for (int u = 0; u < 2; ++u) sees[u] = DECODE ? keys : min(keys, first_pos + token_of(min(2 * t4 + u, cols - 1)) + 1);
   const int all_see = DECODE ? keys : min(keys, first_pos + token_of(0) + 1);
 
-  float m[2] = {-INFINITY, -INFINITY}, ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, L[2][2] = {{0.f, 0.f}, {0.f, 0.f}};     // L[half][column]: sums of weight times level 8
+  float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, L[2][2] = {{0.f, 0.f}, {0.f, 0.f}};     // L[half][column]: sums of weight times level 8
   float O[8][4];                                   // O[4 half + i]: dimensions 64 half + 8 g + 2 i and + 1
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -359,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   const int koff = key_g * kData + ((t4 ^ ((g >> 1) & 2)) << 4);
   const int voff = kOffV + (((g >> 1) ^ (t4 & 2)) << 4) + (g & 1) * 8;
 
+  bool first = true;
   const auto tile = [&](auto edge, const uint8_t* st, int p0) {
     constexpr bool EDGE = decltype(edge)::value;
     float x[2][4];
@@ -400,13 +403,14 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 2; ++r) vp[u][r] = *reinterpret_cast<const uint2*>(st + kOffVP + (u * 16 + 8 * r + key_g) * kParams);
-    float top[2] = {fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]))};
+    float top[2] = {max3(fmaxf(x[0][0], x[0][2]), x[1][0], x[1][2]), max3(fmaxf(x[0][1], x[0][3]), x[1][1], x[1][3])};
     float s_top = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) s_top = fmaxf(s_top, fmaxf(scale_of<BF16>(vp[u][r].x), scale_of<BF16>(vp[u][r].y)));      // (fmaxf passes over a NaN)
-    if (__any_sync(0xFFFFFFFFu, top[0] > kLag || top[1] > kLag || m[0] == -INFINITY || m[1] == -INFINITY || s_top > top_scale)) {
+      for (int r = 0; r < 2; ++r) s_top = max3(s_top, scale_of<BF16>(vp[u][r].x), scale_of<BF16>(vp[u][r].y));      // (a NaN is passed over)
+    // The first tile sets the reference.  (What a column sees is a beginning of the keys: one that sees nothing of the first tile sees nothing at all.)
+    if (first || __any_sync(0xFFFFFFFFu, top[0] > kLag || top[1] > kLag || s_top > top_scale)) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
@@ -415,15 +419,14 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
       float far[2], same = 1.f;                    // what the sums so far are multiplied by
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float n = fmaxf(m[h], top[h] + ref[h]), r = n == -INFINITY ? 0.f : n;
-        far[h] = m[h] == n ? 1.f : exp2_fast(m[h] - n);      // 0 ahead of the first tile
+        const float by = first ? (top[h] == -INFINITY ? 0.f : top[h]) : fmaxf(top[h], 0.f);
+        far[h] = first ? 0.f : exp2_fast(-by);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          x[u][h] -= r - ref[h];
-          x[u][2 + h] -= r - ref[h];
+          x[u][h] -= by;
+          x[u][2 + h] -= by;
         }
-        m[h] = n;
-        ref[h] = r;
+        ref[h] += by;
         l[h] *= far[h];
         L[0][h] *= far[h];
         L[1][h] *= far[h];
@@ -496,6 +499,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
       __syncwarp();
     }
     if (p0 + kTile > all_see) tile(std::true_type(), st, p0); else tile(std::false_type(), st, p0);
+    first = false;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   }
   if (lane < 4) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) { fx.m[warp][2 * lane + h] = m[h]; fx.l[warp][2 * lane + h] = l[h]; }
+    for (int h = 0; h < 2; ++h) { fx.m[warp][2 * lane + h] = l[h] == 0.f ? -INFINITY : ref[h]; fx.l[warp][2 * lane + h] = l[h]; }
   }
   __syncthreads();
   const auto finish = [&](int c, int d, float o, float sum, float top) {
@@ -608,12 +612,18 @@ namespace {
 constexpr int kResident[4][2] = {{296, 592}, {148, 296}, {71, 142}, {33, 66}};   // clusters of 1, 2, 4, 8 CTAs that are resident with rings of 4 and 2 tiles
 constexpr int kMostParts = 16;
 struct Split { int csize, stages, parts; };
+// `keys`: the most that a sequence may see; a unit: eight columns of a key/value head of a sequence.  A CTA for every 128 keys (a tile per warp) as
+// long as all clusters are resident with the short rings, and the long rings where they stay so.  Where clusters of eight leave half of
+// the chip idle, a sequence goes over several of them, down to 128 keys a CTA, and a second kernel adds their shares (3 us).  8 key/value
+// heads, us, over one cluster, two and four: 2048 keys 7.8, 9.0, 9.0; 4000 9.7, 10.4, 9.2; 8000 12.3, 12.3, 10.3; 32000 34, 27, 18.7 (over eight
+// with short rings 20.0).  Finer splits of a chip that is full lose what the CTAs' beginnings and ends cost: 64 x 4000 keys 77 with one CTA a
+// unit, 81 with two.
 Split split(int64_t units, int64_t keys) {
   Split s = {1, 2, 1};
   int row = 0;
   while (row < 3 && units <= kResident[row + 1][1] && keys > (int64_t)s.csize * kWarps * kTile) { s.csize *= 2; ++row; }
-  if (row == 3 && keys >= 8 * 1024)
-    while (s.parts < kMostParts && units * s.parts * 2 <= kResident[3][1] && keys >= 8 * s.parts * 2 * 256) s.parts *= 2;
+  if (row == 3 && keys >= 4096)
+    while (s.parts < kMostParts && units * s.parts * 2 <= kResident[3][0] && keys >= 8 * s.parts * 2 * 128) s.parts *= 2;
   if (units * s.parts <= kResident[row][0]) s.stages = 4;
   return s;
 }
