@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   grid_launch_dependents();
   grid_dependency_wait();
   cg::cluster_group cl = cg::this_cluster();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, csize = gridDim.x / a.parts, rank = blockIdx.x % csize;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), csize = gridDim.x / a.parts, rank = blockIdx.x % csize;
   const int kvh = blockIdx.y / a.groups, group = blockIdx.y % a.groups, b = blockIdx.z;
   const int R = a.heads / a.cache.kv_heads;
   const int t_first = DECODE ? b : a.cu[b], n_tokens = DECODE ? 1 : a.cu[b + 1] - t_first;
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel
   const auto page_of = [&](int key, int& row) {
     const int at = a.shift >= 0 ? key >> a.shift : (int)((unsigned)key / (unsigned)a.cache.block);
     row = key - at * a.cache.block;
-    return table[at];
+    return __shfl_sync(0xFFFFFFFFu, table[at], 0);
   };
   auto load = [&](int t, int stage) {
     if (t < t1) {
