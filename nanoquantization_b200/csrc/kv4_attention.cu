@@ -135,9 +135,11 @@ __device__ __forceinline__ float operand(const Half& hx, const Half& hy, uint4& 
   return __uint_as_float((e - 8u) << 23);
 }
 
-// STAGES: tiles of a warp's ring (see split()).  DECODE: one token per sequence whose own key and value are made here.
-template <bool BF16, bool DECODE, int STAGES>
-__global__ void __launch_bounds__(kThreads, STAGES == 2 ? 4 : 2) kv4_rows_kernel(const __grid_constant__ Args a) {
+// CTAS: of an SM (see split()); they share its registers and its room for rings.  DECODE: one token per sequence whose own key and value are made here.
+__host__ __device__ constexpr int stages_of(int ctas) { return ctas == 4 ? 2 : ctas == 3 ? 3 : 4; }
+template <bool BF16, bool DECODE, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_constant__ Args a) {
+  constexpr int STAGES = stages_of(CTAS);
   constexpr int kRing = ring_bytes(STAGES);
   // A query of a float16 model that comes from float goes in as two numbers: its rounding is half of the error otherwise (3500 keys: 4.1e-4 in
   // the 2-norm with one, 2.9e-4 with two, 2.1e-4 of them the result's own rounding), for 8 % of the time.  Given queries are exact, and
@@ -608,31 +610,42 @@ int kv4::add_shares(const float* shares, uint16_t* out, int64_t rows, int parts,
 
 namespace {
 
-// How a call is split: CTAs of a cluster, clusters of a sequence, tiles of a warp's ring.
-constexpr int kResident[4][2] = {{296, 592}, {148, 296}, {71, 142}, {33, 66}};   // clusters of 1, 2, 4, 8 CTAs that are resident with rings of 4 and 2 tiles
+// How a call is split: CTAs of a cluster, CTAs that share an SM, clusters of a sequence.  Clusters of 1, 2, 4, 8 CTAs that are resident with 2, 3
+// and 4 CTAs to an SM:
+constexpr int kResident[4][3] = {{296, 444, 592}, {148, 222, 296}, {71, 104, 142}, {33, 48, 66}};
 constexpr int kMostParts = 16;
-struct Split { int csize, stages, parts; };
-// `keys`: the most that a sequence may see; a unit: eight columns of a key/value head of a sequence.  A CTA for every 128 keys (a tile per warp) as
-// long as all clusters are resident with the short rings, and the long rings where they stay so.  Where clusters of eight leave half of
-// the chip idle, a sequence goes over several of them, down to 128 keys a CTA, and a second kernel adds their shares (3 us).  8 key/value
-// heads, us, over one cluster, two and four: 2048 keys 7.8, 9.0, 9.0; 4000 9.7, 10.4, 9.2; 8000 12.3, 12.3, 10.3; 32000 34, 27, 18.7 (over eight
-// with short rings 20.0).  Finer splits of a chip that is full lose what the CTAs' beginnings and ends cost: 64 x 4000 keys 77 with one CTA a
-// unit, 81 with two.
+struct Split { int csize, ctas, parts; };
+// `keys`: the most that a sequence may see; a unit: eight columns of a key/value head of a sequence.
+// The fewer CTAs share an SM, the more registers each has: a CTA per 128 keys (a tile per warp) as long as the clusters are resident three to an SM,
+// and two to an SM where they still are.  Units of 1500 keys, us, with 2, 3, 4 to an SM: 192 (clusters of two) 28.5, 18.8, 21.8; 256 (of 2000) 25.1,
+// 31.1, 37.3; 360 37.1, 26.6, 33.0.  Four to an SM is for what then takes one turn instead of two: 512 of 4000 80, 87, 75, and where turns
+// are many; 880 units 55.7, 48.9, 54.1; 2048 of 800 87, 72.7, 70.9.
+// Where clusters of eight leave half of the chip idle, a sequence goes over several of them, down to 128 keys a CTA, and a second kernel adds their
+// shares (3 us).  8 key/value heads, over one cluster, two and four: 2048 keys 7.8, 9.0, 9.0; 4000 9.7, 10.4, 9.2; 8000 12.3, 12.3, 10.3;
+// 32000 34, 27, 18.7.
 Split split(int64_t units, int64_t keys) {
-  Split s = {1, 2, 1};
+  Split s = {1, 4, 1};
   int row = 0;
   while (row < 3 && units <= kResident[row + 1][1] && keys > (int64_t)s.csize * kWarps * kTile) { s.csize *= 2; ++row; }
   if (row == 3 && keys >= 4096)
     while (s.parts < kMostParts && units * s.parts * 2 <= kResident[3][0] && keys >= 8 * s.parts * 2 * 128) s.parts *= 2;
-  if (units * s.parts <= kResident[row][0]) s.stages = 4;
+  const auto turns = [&](int ctas) { return (units * s.parts + kResident[row][ctas - 2] - 1) / kResident[row][ctas - 2]; };
+  if (turns(2) == 1) s.ctas = 2;
+  else if (turns(3) * 4 < turns(4) * 5) s.ctas = 3;
   return s;
 }
 
 int groups_of(int64_t tokens, int64_t heads, int64_t kv_heads) { return (int)((tokens * (heads / kv_heads) + kCols - 1) / kCols); }
 
-template <bool BF16, bool DECODE, int STAGES> int launch_stages(const Args& a, int csize, int64_t batch, cudaStream_t st) {
-  constexpr auto kernel = kv4_rows_kernel<BF16, DECODE, STAGES>;
-  constexpr int smem = smem_bytes(STAGES);
+// Units that have columns: sequences shorter than the longest have fewer, and half a unit each is lost at their ends.
+int64_t units_of(int64_t batch, int64_t tokens, int64_t groups, int64_t heads, int64_t kv_heads) {
+  const int64_t full = batch * groups, some = tokens * (heads / kv_heads) / kCols + (batch + 1) / 2;
+  return kv_heads * (tokens > batch && some < full ? some : full);
+}
+
+template <bool BF16, bool DECODE, int CTAS> int launch_ctas(const Args& a, int csize, int64_t batch, cudaStream_t st) {
+  constexpr auto kernel = kv4_rows_kernel<BF16, DECODE, CTAS>;
+  constexpr int smem = smem_bytes(stages_of(CTAS));
   if (!allow_smem<kernel>(smem)) return NQB200_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(csize * a.parts), (unsigned)(a.cache.kv_heads * a.groups), (unsigned)batch);
@@ -652,10 +665,12 @@ template <bool BF16, bool DECODE, int STAGES> int launch_stages(const Args& a, i
   return NQB200_OK;
 }
 template <bool BF16, bool DECODE> int launch_t(Args& a, int64_t batch, int64_t tokens, int64_t keys, cudaStream_t st) {
-  const Split s = split((int64_t)a.cache.kv_heads * a.groups * batch, keys);
+  const Split s = split(units_of(batch, tokens, a.groups, a.heads, a.cache.kv_heads), keys);
   a.parts = s.parts;
   a.shift = (a.cache.block & (a.cache.block - 1)) == 0 ? __builtin_ctz((unsigned)a.cache.block) : -1;
-  const int rc = s.stages == 4 ? launch_stages<BF16, DECODE, 4>(a, s.csize, batch, st) : launch_stages<BF16, DECODE, 2>(a, s.csize, batch, st);
+  const int rc = s.ctas == 2   ? launch_ctas<BF16, DECODE, 2>(a, s.csize, batch, st)
+                 : s.ctas == 3 ? launch_ctas<BF16, DECODE, 3>(a, s.csize, batch, st)
+                               : launch_ctas<BF16, DECODE, 4>(a, s.csize, batch, st);
   if (rc != NQB200_OK || s.parts == 1) return rc;
   return add_shares(a.shares, a.out, tokens * a.heads, s.parts, BF16, st);
 }
@@ -663,7 +678,7 @@ template <bool DECODE> int launch(Args& a, int64_t batch, int64_t tokens, int64_
   return dtype == NQB200_BF16 ? launch_t<true, DECODE>(a, batch, tokens, keys, st) : launch_t<false, DECODE>(a, batch, tokens, keys, st);
 }
 size_t scratch_bytes_of(int64_t batch, int64_t tokens, int64_t max_len, int64_t keys, int64_t heads, int64_t kv_heads) {
-  const Split s = split(kv_heads * groups_of(max_len, heads, kv_heads) * batch, keys);
+  const Split s = split(units_of(batch, tokens, groups_of(max_len, heads, kv_heads), heads, kv_heads), keys);
   return s.parts > 1 ? (size_t)(tokens * heads * s.parts * kShare) * sizeof(float) : 0;
 }
 bool heads_fit(int64_t heads, int64_t kv_heads) { return kv_heads > 0 && kv_heads <= 4096 && heads > 0 && heads <= 65535 && heads % kv_heads == 0; }

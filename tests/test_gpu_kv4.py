@@ -609,3 +609,15 @@ def test_copies_of_pools_that_do_not_fit():
             copy_pages([a], src, dst)
     with pytest.raises(RuntimeError, match="bad shape"):
         copy_pages([torch.zeros(4, 0, device=DEV)], [0], [1])
+
+
+# rings that wrap with remainders for every number of CTAs on an SM: 192, 256, 360, 512 and 640 units of key/value heads
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,keys,kv_heads,heads", [(24, 700, 8, 16), (32, 600, 8, 8), (45, 500, 8, 32), (64, 400, 8, 64), (80, 300, 8, 24)], ids=str)
+@torch.no_grad()
+def test_decode_of_many_sequences(B, keys, kv_heads, heads, dtype):
+    from nanoquantization_b200.layers import kv4
+    ctx, block = tuple(keys - 7 * i % (keys - 1) for i in range(B)), 64
+    kc, vc, table, rows, qkv, qw, kw, cs, at, positions = _decode_inputs(ctx, kv_heads, heads, block, dtype)
+    got = kv4.decode_attention(qkv, qw, kw, cs, positions, heads, kv_heads, 1e-6, kc, vc, table, torch.tensor(ctx, dtype=torch.int32, device=DEV), at)
+    _decode_check(got, ctx, kv_heads, heads, block, dtype, kc, vc, rows, qkv, qw, kw, cs, positions)
