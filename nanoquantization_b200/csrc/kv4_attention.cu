@@ -375,6 +375,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const Lifted la = lift(wa[j], magic), lb = lift(wb[j], magic);
+        if (CTAS == 4) {                           // (again from shared memory rather than in 16 registers)
+          const uint4 v = *reinterpret_cast<const uint4*>(&fx.q[g][64 * (j & 1) + 16 * t4 + 8 * (j >> 1)]);
+          qf[j][0] = v.x; qf[j][1] = v.y; qf[j][2] = v.z; qf[j][3] = v.w;
+        }
         if (j < 2) mma_from(c[j], start[j], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
         else mma(c[j & 1], la.v[0], lb.v[0], la.v[1], lb.v[1], qf[j][0], qf[j][1]);
         mma(c[j & 1], la.v[2], lb.v[2], la.v[3], lb.v[3], qf[j][2], qf[j][3]);
