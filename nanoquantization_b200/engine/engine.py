@@ -135,9 +135,22 @@ class PagedKVCache:
             self.v = [None if s is None else pool(s.kv_heads, s.v_dim) for s in layout.kv]
         self.block_size, self.bits = block_size, bits
 
+    def copy(self, pairs: list[tuple[int, int]]) -> None:
+        """Blocks ``(from, to)``, in every layer."""
+        _copy_rows([p for p in self.k + self.v if p is not None], pairs)
+
     def write(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         self.k[layer].view(-1, *k.shape[1:]).index_copy_(0, slots, k)
         self.v[layer].view(-1, *v.shape[1:]).index_copy_(0, slots, v)
+
+
+def _copy_rows(pools: list[torch.Tensor], pairs: list[tuple[int, int]]) -> None:
+    sources, targets = [a for a, _ in pairs], [b for _, b in pairs]
+    if pools[0].is_cuda:
+        copy_pages(pools, sources, targets)
+    else:
+        for p in pools:
+            p[targets] = p[sources]
 
 
 class StatePool:
@@ -155,6 +168,9 @@ class StatePool:
                 return False
             seq.slot = self.free.popleft()
         return True
+
+    def copy(self, source: int, target: int) -> None:
+        _copy_rows([p for run in self.states for p in run.values()], [(source, target)])
 
     def release(self, seq: Sequence) -> None:
         if seq.slot is not None:
@@ -327,7 +343,7 @@ class LLMEngine:
         self.states = StatePool(self.layout, max_batch + 1, self.device)
         self.scratch_block, self.scratch_slot = num_blocks, max_batch
         self.blocks = BlockManager(num_blocks, block_size)
-        self.blocks.copy = self._copy_blocks
+        self.blocks.copy = self.cache.copy      # (not a method of the engine: it has to go when its last user does, not when garbage is collected)
         self.scheduler = Scheduler(self.blocks, max_batch, max_prefill_tokens, prefill_portion, self.states)
         self.use_cuda_graph = use_cuda_graph
         self.paged_attention = self._probe_flash_attn() if model.delegates_attention and block_size % 256 == 0 and kv_bits == 16 else None
@@ -353,16 +369,6 @@ class LLMEngine:
             return None
 
     # --------------------------------------------------------------------- steps
-    def _copy_rows(self, pools: list[torch.Tensor], pairs: list[tuple[int, int]]) -> None:
-        if self.device.type == "cuda":
-            copy_pages(pools, [a for a, _ in pairs], [b for _, b in pairs])
-        else:
-            for p in pools:
-                p[[b for _, b in pairs]] = p[[a for a, _ in pairs]]
-
-    def _copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
-        self._copy_rows([p for p in self.cache.k + self.cache.v if p is not None], pairs)
-
     def _forward(self, batch: StepBatch, decode: bool, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         return self.model.forward_step(batch, lambda run: LayerStep(self, run, batch, decode), rows)
 
@@ -496,7 +502,7 @@ class LLMEngine:
         if self.layout.recurrent and s.slot is not None:
             if not self.states.ensure(t):
                 raise RuntimeError(f"no state slot is free for a fork of sequence {s.seq_id}")
-            self._copy_rows([p for run in self.states.states for p in run.values()], [(s.slot, t.slot)])
+            self.states.copy(s.slot, t.slot)
         self.blocks.share(s, t)
         return t
 

@@ -217,3 +217,21 @@ def test_a_fork_holds_what_its_sequence_holds():
     assert torch.equal(engine.cache.k[0][t.blocks[1]], before[s.blocks[1]])
     engine.drop(s), engine.drop(t)
     assert sorted(engine.blocks.free) == list(range(6))
+
+
+def test_an_engine_goes_with_its_last_user():
+    """No cycle of references: an engine that garbage collection took in the middle of another's graph capture would end that capture."""
+    import gc
+    import weakref
+    from nanoquantization_b200.engine import LLMEngine
+    from nanoquantization_b200.models.qwen3_quantized import Qwen3QuantizedForCausalLM
+    model = Qwen3QuantizedForCausalLM(1, 64, 256, 2, 1, 32, 128, 4, 128, 128, device="cpu", dtype=torch.float16)
+    gc.disable()
+    try:
+        for bits in (16, 4):
+            engine = LLMEngine(model, num_blocks=2, block_size=16, max_batch=2, kv_bits=bits)
+            gone = weakref.ref(engine)
+            del engine
+            assert gone() is None
+    finally:
+        gc.enable()
