@@ -39,11 +39,12 @@ __device__ __forceinline__ float divided(float a, float b, float reciprocal) {
   const float t = a * reciprocal;
   return fmaf(fmaf(-t, b, a), reciprocal, t);
 }
-// Scale and offset of a group from its smallest and largest value: two 16-bit numbers, scale first.
+// Scale and offset of a group from its smallest and largest value: two 16-bit numbers, scale first.  (An offset that its rounding put above the
+// largest value leaves a scale of 0: all levels are the offset.)
 template <bool BF16> __device__ __forceinline__ uint32_t group_params(float lo, float hi) {
   const uint16_t m = float_to_raw16<BF16>(lo);
   const float d = hi - raw16_to_float<BF16>(m);
-  const uint16_t s = float_to_raw16<BF16>(fabsf(d) < INFINITY ? divided(d, 15.f, 1.f / 15.f) : __int_as_float(0x7FC00000));
+  const uint16_t s = float_to_raw16<BF16>(fabsf(d) < INFINITY ? fmaxf(divided(d, 15.f, 1.f / 15.f), 0.f) : __int_as_float(0x7FC00000));
   return (uint32_t)s | ((uint32_t)m << 16);
 }
 template <bool BF16> __device__ __forceinline__ float scale_of(uint32_t params) { return raw16_to_float<BF16>((uint16_t)(params & 0xFFFF)); }

@@ -21,6 +21,11 @@
 //
 // Scores come out relative to a reference, which moves only when one is 8 (in log2 units) above it, found by one vote per 32 keys.  The warps meet in
 // shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
+//
+// 64 sequences of 3500 keys on average, 64 heads over 8, bfloat16 (263 MB, 40 us at the copy rate): 74 us; float16 80; 45 of 1250, 32 heads over 8 (69
+// MB, 10.6 us) 26.5; one of 32000 18; one of 37 6.3.  The bytes come in at 3.6 TB/s at most: issue slots are 59 % busy (697 warp
+// instructions for 32 keys, of them 208 to take nibbles and parameters apart, 107 float arithmetic, 64 packed half, 32 products), the ALU
+// 51 %, the tensor pipe 21 %, DRAM 40 %, and CTAs of unequal sequences end at different times (IPC 2.3 while they run, 1.9 over all).
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "kv4_attention.cuh"
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
   constexpr int STAGES = stages_of(CTAS);
   constexpr int kRing = ring_bytes(STAGES);
   // A query of a float16 model that comes from float goes in as two numbers: its rounding is half of the error otherwise (3500 keys: 4.1e-4 in
-  // the 2-norm with one, 2.9e-4 with two, 2.1e-4 of them the result's own rounding), for 8 % of the time.  Given queries are exact, and
+  // the 2-norm with one, 3.0e-4 with two, 2.1e-4 of them the result's own rounding), for 8 % of the time.  Given queries are exact, and
   // bfloat16's results are coarser.
   constexpr bool kRest = DECODE && !BF16;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
       const int page = page_of(p0, row0);
       const bool whole = p0 + kTile <= stored && (unsigned)page < (unsigned)a.cache.pages;
       // a whole tile of one page, a whole tile of two pages (16 rows lie in one), and any other: 64 sequences of 4000 keys of 8 heads, us,
-      // by the first way, the second and the third: pages of 256 tokens 75, 80, 90; of 16 tokens -, 83, 94
+      // by the first way, the second and the third: pages of 256 tokens 73.6, 77.0, 85.6; of 16 tokens -, 79.2, 87.8
       int row1 = 0, page1 = -1;
       if (whole && a.cache.block % kTile != 0) page1 = page_of(p0 + 16, row1);
       if (whole && a.cache.block % kTile == 0) {
@@ -625,7 +630,7 @@ struct Split { int csize, ctas, parts; };
 // 31.1, 37.3; 360 37.1, 26.6, 33.0.  Four to an SM is for what then takes one turn instead of two: 512 of 4000 80, 87, 75, and where turns
 // are many; 880 units 55.7, 48.9, 54.1; 2048 of 800 87, 72.7, 70.9.
 // Where clusters of eight leave half of the chip idle, a sequence goes over several of them, down to 128 keys a CTA, and a second kernel adds their
-// shares (3 us).  8 key/value heads, over one cluster, two and four: 2048 keys 7.8, 9.0, 9.0; 4000 9.7, 10.4, 9.2; 8000 12.3, 12.3, 10.3;
+// shares (3 us).  8 key/value heads, over one cluster, two and four: 2048 keys 7.8, 9.6, 9.0; 4000 9.7, 10.4, 9.2; 8000 12.3, 12.3, 10.3;
 // 32000 34, 27, 18.7.
 Split split(int64_t units, int64_t keys) {
   Split s = {1, 4, 1};

@@ -2,6 +2,10 @@
 //
 // Both are bound by memory: a token's projections in (256 bytes a head), its queries out and 144 bytes per key/value head stored.
 // Eight lanes per (token, head), every access 16 bytes wide (8 where a row of nibbles is written).
+//
+// 4096 tokens of 32 + 8 + 8 heads, bfloat16 (91 MB, 13.9 us at the copy rate): 23.4 us, 3.9 TB/s; 100 tokens of 16 + 8 + 8 2.6 us.  Issue slots are 64 %
+// busy (308 warp instructions for four heads), the ALU 48 %.  16 lanes a head with half the width took 38.5, this with plain arithmetic
+// and conversions 32.8, two heads per eight lanes 38.3 (88 registers a thread instead of 48).  Read-back of 4096 rows: 8.9 us (43 MB).
 #include "kv4.cuh"
 
 namespace nqb200 {

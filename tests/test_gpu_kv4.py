@@ -135,6 +135,32 @@ def test_store_of_special_rows(dtype):
     assert torch.isfinite(got[6:]).all() and ((got[6:].double() - y).abs() <= edge).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@torch.no_grad()
+def test_values_far_from_zero_with_a_small_range(dtype):
+    """Ranges below the offset's rounding: the offset alone stands for them, in every way of reading."""
+    from nanoquantization_b200.layers import kv4
+    n, cs = 20, ref.angles(32, DEV)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    qkv = torch.zeros(n, 3 * D, device=DEV)
+    qkv[:, :D] = torch.randn(n, D, generator=g, device=DEV)
+    qkv[:, D:2 * D] = 100 + torch.rand(n, D, generator=g, device=DEV) * 0.01      # after its norm, 1 and little around it
+    qkv[:, 2 * D:] = 100 + torch.rand(n, D, generator=g, device=DEV) * 0.01
+    qkv = qkv.to(dtype)
+    w, rows, i32 = torch.ones(D, device=DEV).to(dtype), torch.arange(n, device=DEV), lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    w = (w + 0.001 * torch.arange(D, device=DEV) / D).to(dtype)
+    kc, vc = kv4.new_cache(2, 16, 1, DEV)
+    q = kv4.qknorm_rope_store(qkv, w, w, cs, torch.zeros(n, dtype=torch.int64, device=DEV), 1, 1, 1e-6, kc, vc, rows)
+    k, v = (ref.rows_of(c, rows.tolist(), 16, dtype) for c in (kc, vc))
+    assert (ref.rows_of(kc, rows.tolist(), 16, dtype) - ref.norm_rope(qkv.double()[:, None, D:2 * D], w, cs, torch.zeros(n, dtype=torch.int64, device=DEV))).abs().max() <= 2 * ref.unit(dtype)
+    scales = torch.stack([c[..., 16 * 64:].unflatten(-1, (16, 8)).contiguous().view(dtype)[..., ::2].float() for c in (kc, vc)])
+    assert (scales >= 0).all()
+    table = i32(0, 1)[None]
+    _close(kv4.prompt_attention(q, 1, kc, vc, table, i32(0, n), i32(0), [n], [0]), ref.attend(q.double().view(n, 1, D), k, v, 0).flatten(1), dtype)
+    got = kv4.decode_attention(qkv[n - 1:], w, w, cs, torch.zeros(1, dtype=torch.int64, device=DEV), 1, 1, 1e-6, kc, vc, table, i32(n), rows[n - 1:])
+    _close(got, ref.attend(q[n - 1:].double().view(1, 1, D), k, v, n - 1).flatten(1), dtype)
+
+
 # ------------------------------------------------------------------ decode
 # edges of tiles and pages, groups of heads below, at and above eight, long ones alone, many at once
 DECODE = [((1,), 1, 1, 16), ((2, 16, 17, 64, 65), 2, 8, 16), ((5, 500, 1025), 2, 2, 256), ((129, 3, 31, 32, 33), 3, 48, 48), ((33,) * 70, 8, 32, 256),
