@@ -3,7 +3,8 @@
 // Both are bound by memory: a token's projections in (256 bytes a head), its queries out and 144 bytes per key/value head stored.
 // Eight lanes per (token, head), every access 16 bytes wide (8 where a row of nibbles is written).
 //
-// 4096 tokens of 32 + 8 + 8 heads, bfloat16 (91 MB, 13.9 us at the copy rate): 23.4 us, 3.9 TB/s; 100 tokens of 16 + 8 + 8 2.6 us.  Issue slots are 64 %
+// 4096 tokens of 32 + 8 + 8 heads, bfloat16 (91 MB, 13.9 us at the copy rate): 22.3 us, 4.1 TB/s (five blocks to an SM 23.4, four 25.0); 100
+// tokens of 16 + 8 + 8 2.7.  Issue slots are 64 %
 // busy (308 warp instructions for four heads), the ALU 48 %.  16 lanes a head with half the width took 38.5, this with plain arithmetic
 // and conversions 32.8, two heads per eight lanes 38.3 (88 registers a thread instead of 48).  Read-back of 4096 rows: 8.9 us (43 MB).
 #include "kv4.cuh"
@@ -26,7 +27,7 @@ struct StoreArgs {
 };
 
 template <bool BF16, bool WIDE>
-__global__ void __launch_bounds__(256, 5) kv4_store_kernel(const __grid_constant__ StoreArgs a) {
+__global__ void __launch_bounds__(256, 6) kv4_store_kernel(const __grid_constant__ StoreArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int m = threadIdx.x & 7, Hq = a.heads, Hkv = a.cache.kv_heads, per = Hq + 2 * Hkv;
