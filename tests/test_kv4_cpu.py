@@ -235,3 +235,68 @@ def test_an_engine_goes_with_its_last_user():
             assert gone() is None
     finally:
         gc.enable()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_blocks_hold_what_their_sequences_wrote(seed):
+    """Random growth, forks, copies, reclaims and releases over a pool whose contents are tracked."""
+    import random
+    from nanoquantization_b200.engine import BlockManager, Sequence
+    rng, size, total = random.Random(seed), 4, 24
+    m = BlockManager(total, size)
+    memory = [[None] * size for _ in range(total)]
+
+    def copy(pairs):
+        assert len({b for _, b in pairs}) == len(pairs) and {a for a, _ in pairs}.isdisjoint(b for _, b in pairs)      # as copy_pages asks
+        before = [list(x) for x in memory]
+        for a, b in pairs:
+            memory[b] = before[a]
+    m.copy = copy
+    live, next_id = [], 0
+
+    def holders(b):
+        return sum(b in s.blocks for s in live)
+    for _ in range(600):
+        what = rng.random()
+        if what < 0.15 or not live:
+            live.append(Sequence(next_id, [], 1 << 30))
+            next_id += 1
+        elif what < 0.3:
+            s = rng.choice(live)
+            t = Sequence(next_id, list(s.prompt), 1 << 30)
+            t.computed = s.computed
+            next_id += 1
+            m.share(s, t)
+            live.append(t)
+        elif what < 0.4:
+            s = live.pop(rng.randrange(len(live)))
+            m.release(s)
+        elif what < 0.45:
+            s = rng.choice(live)
+            s.first = max(getattr(s, "first", 0), rng.randint(0, s.computed) // size * size)
+            m.reclaim(s, s.first)
+        else:      # a step of one or several sequences, each with its next tokens
+            step = []
+            for s in rng.sample(live, rng.randint(1, len(live))):
+                n = rng.choice([1, 1, 2, 5])
+                if m.ensure(s, s.computed + n + rng.choice([0, 1])):
+                    step.append((s, n))
+            m.flush()
+            for s, n in step:
+                for _ in range(n):
+                    s.prompt.append((s.seq_id, rng.random()))
+                    block = s.blocks[s.computed // size]
+                    assert block >= 0 and holders(block) == 1
+                    memory[block][s.computed % size] = s.prompt[-1]
+                    s.computed += 1
+        if not m.copies:
+            for s in live:
+                for p in range(s.computed):
+                    b = s.blocks[p // size]
+                    assert b < 0 or memory[b][p % size] == s.prompt[p]
+        used = {b for s in live for b in s.blocks if b >= 0}
+        assert used.isdisjoint(m.free) and len(used) + len(m.free) == total and len(set(m.free)) == len(m.free)
+        assert all(holders(b) == n + 1 for b, n in m.shared.items()) and all(holders(b) == 1 for b in used if b not in m.shared)
+    for s in live:
+        m.release(s)
+    assert sorted(m.free) == list(range(total)) and not m.shared
