@@ -250,6 +250,11 @@ def check_mixer_status() -> None:
             check_mixers(status)
 
 
+# (absent from a build of torch without CUDA)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 class on_device:
     """Makes a GPU the current one for a call, and gives its current stream."""
     __slots__ = ("index", "before")
@@ -258,10 +263,10 @@ class on_device:
         self.index = index
 
     def __enter__(self) -> int:
-        self.before = torch._C._cuda_getDevice()
+        self.before = _current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+        return _current_stream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:

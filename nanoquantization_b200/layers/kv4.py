@@ -59,14 +59,15 @@ def _projections(qkv, q_weight, k_weight, cos_sin, positions, num_q_heads, kv_he
         raise ValueError(f"{num_q_heads} query heads over {kv_heads} do not go with a cache of {cache.kv_heads} key/value heads")
     if len(shape) != 2 or shape[1] != (num_q_heads + 2 * kv_heads) * DIM or qkv.stride(1) != 1:
         raise ValueError(f"qkv must be [tokens, {(num_q_heads + 2 * kv_heads) * DIM}] with unit stride along a row, got {tuple(shape)}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype is not dtype or w.shape != (DIM,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {DIM}")
+    if q_weight.dtype is not dtype or k_weight.dtype is not dtype or q_weight.numel() != DIM or k_weight.numel() != DIM or not (q_weight.is_contiguous() and
+                                                                                                                              k_weight.is_contiguous()):
+        raise ValueError(f"q_weight and k_weight must be contiguous {dtype} tensors of {DIM}")
     if cos_sin.dtype is not torch.float32 or cos_sin.shape[-1] != DIM or not cos_sin.is_contiguous():
         raise ValueError(f"cos_sin must be a contiguous float32 tensor [..., {DIM}]")
     tokens = shape[:1]
-    _ints("positions", positions, torch.int64, tokens)
-    _ints("rows", rows, torch.int64, tokens)
+    if positions.dtype is not torch.int64 or rows.dtype is not torch.int64 or positions.shape != tokens or rows.shape != tokens or not (positions.is_contiguous() and
+                                                                                                                                      rows.is_contiguous()):
+        raise ValueError(f"positions and rows must be contiguous int64 tensors of {shape[0]}")
     return _lib.dtype_code(dtype)
 
 
@@ -116,12 +117,15 @@ def decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.
     lib = _lib.load()
     with _lib.on_device(dev) as stream:
         out = qkv.new_empty((B, num_q_heads * DIM))
-        need = lib.nqb200_kv4_decode_scratch_bytes(width, cache.block_size, B, num_q_heads, num_kv_heads)
-        scratch = k_cache.new_empty(need) if need else None
-        status = lib.nqb200_kv4_decode_attention(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM,
-                                                 positions.data_ptr(), rows.data_ptr(), cache, table.data_ptr(), width, ctx.data_ptr(), out.data_ptr(), B,
-                                                 num_q_heads, DIM ** -0.5 if scale is None else scale, eps, code, scratch.data_ptr() if need else None, need,
-                                                 _lib.cache_status(dev), stream)
+        call = [qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM, positions.data_ptr(),
+                rows.data_ptr(), cache, table.data_ptr(), width, ctx.data_ptr(), out.data_ptr(), B, num_q_heads, DIM ** -0.5 if scale is None else scale, eps, code,
+                None, 0, _lib.cache_status(dev), stream]
+        status = lib.nqb200_kv4_decode_attention(*call)
+        if status == 5:        # a few long sequences, whose clusters' shares need room (asking ahead would cost every other call)
+            need = lib.nqb200_kv4_decode_scratch_bytes(width, cache.block_size, B, num_q_heads, num_kv_heads)
+            scratch = k_cache.new_empty(need)
+            call[18], call[19] = scratch.data_ptr(), need
+            status = lib.nqb200_kv4_decode_attention(*call)
     _lib.check(status)
     return out
 
