@@ -23,7 +23,7 @@
 // shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
 //
 // 64 sequences of 3500 keys on average, 64 heads over 8, bfloat16 (263 MB, 40 us at the copy rate): 74 us; float16 80; 45 of 1250, 32 heads over 8 (69
-// MB, 10.6 us) 26.5; one of 32000 18; one of 37 6.3.  The bytes come in at 3.6 TB/s at most: issue slots are 59 % busy (697 warp
+// MB, 10.6 us) 26.5; one of 32000 17.7; one of 37 6.3.  The bytes come in at 3.6 TB/s at most: issue slots are 59 % busy (697 warp
 // instructions for 32 keys, of them 208 to take nibbles and parameters apart, 107 float arithmetic, 64 packed half, 32 products), the ALU
 // 51 %, the tensor pipe 21 %, DRAM 40 %, and CTAs of unequal sequences end at different times (IPC 2.3 while they run, 1.9 over all).
 #include <cooperative_groups.h>
@@ -593,21 +593,41 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
   cl.sync();                                       // peers may still read this CTA's shared memory
 }
 
-// The shares of a row's clusters, a CTA per (token, query head), in the clusters' order.
+// The shares of a row, a CTA per (token, query head), in their order.  A lane has the maximum and the sum of two of up to 64 shares.
 template <bool BF16>
 __global__ void __launch_bounds__(kDim) kv4_shares_kernel(const float* __restrict__ shares, uint16_t* __restrict__ out, int parts) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int64_t row = blockIdx.x;
   const float* s = shares + row * parts * kShare;
-  float top = -INFINITY, sum = 0.f, o = 0.f;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, s[p * kShare + kDim]);
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float m = s[p * kShare + kDim], f = m == top ? 1.f : exp2f(m - top);
-    o += f * s[p * kShare + threadIdx.x];
-    sum += f * s[p * kShare + kDim + 1];
+  const int lane = threadIdx.x & 31;
+  float m[2], f[2], sum = 0.f, top = -INFINITY, o = 0.f, v[8];       // v: the first shares' sums, under way beside the maxima
+#pragma unroll
+  for (int p = 0; p < 8; ++p) v[p] = p < parts ? s[p * kShare + threadIdx.x] : 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int p = lane + 32 * k;
+    m[k] = p < parts ? s[p * kShare + kDim] : -INFINITY;
+    f[k] = p < parts ? s[p * kShare + kDim + 1] : 0.f;
+    top = fmaxf(top, m[k]);
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float by = m[k] == top ? 1.f : exp2f(m[k] - top);
+    sum += by * f[k];
+    f[k] = by;
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const float by = __shfl_sync(0xFFFFFFFFu, f[0], p);
+    if (p < parts) o += by * v[p];
+  }
+#pragma unroll 8
+  for (int p = 8; p < parts; ++p) o += __shfl_sync(0xFFFFFFFFu, p < 32 ? f[0] : f[1], p & 31) * s[p * kShare + threadIdx.x];
   out[row * kDim + threadIdx.x] = float_to_raw16<BF16>(sum == 0.f ? 0.f : o / sum);
 }
 

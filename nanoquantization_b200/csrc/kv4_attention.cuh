@@ -7,7 +7,7 @@ namespace kv4 {
 
 constexpr int kShare = kDim + 4;      // floats of a row's share of its keys: sums, maximum (log2 units), sum of weights
 
-// out[row] = the sum of the row's shares, in their order, over its sum of weights; 0 where there is no key.
+// out[row] = the sum of the row's shares (64 at most), in their order, over its sum of weights; 0 where there is no key.
 int add_shares(const float* shares, uint16_t* out, int64_t rows, int parts, bool bf16, cudaStream_t st);
 
 bool prompt_umma_faster(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads);

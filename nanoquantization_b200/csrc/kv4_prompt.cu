@@ -97,7 +97,7 @@ __device__ __forceinline__ int tiles_before(const Params& p, int b) {
 
 // A tile of 128 rows of a key/value head: 16 lanes a row, lane 2 m + j takes word 2 m + j, 8 dimensions, 16 bytes out.
 template <bool BF16>
-__global__ void __launch_bounds__(512) kv4_expand_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(512, 3) kv4_expand_kernel(const __grid_constant__ Params p) {
   __shared__ int s_before, s_bad[2];
   __shared__ uint32_t s_top[2];
   grid_launch_dependents();
@@ -641,7 +641,7 @@ int parts_of(int64_t batch, int64_t max_len, int64_t max_ctx, int64_t heads, int
 // Which of the two ways a call takes: the one that is expected to end first, in us, by what 68 calls of either took (16 to 512 tokens of 1 to 32
 // sequences behind 0 to 16000, 2 to 8 query heads per key/value head, 1 and 8 of those; a wrong choice costs 2 us, and up to 10 for
 // long drafts of one key/value head).  Few rows: a CTA per 8 of them goes over the keys.  Many: the pages taken apart, then tiles of
-// 256 rows x 128 keys one after the other.  64 tokens of 32 heads over 8: 7.2 and 16.2 us alone, 27 and 31 behind 2000, 148 and 60 behind 16000.
+// 256 rows x 128 keys one after the other.  64 tokens of 32 heads over 8: 7.2 and 16.2 us alone, 27 and 31 behind 2000, 148 and 56 behind 16000.
 bool prompt_umma_faster(int64_t batch, int64_t tokens, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t heads, int64_t kv_heads) {
   const double rows = (double)tokens * (heads / kv_heads), mean_keys = fmax(1.0, 128.0 * tiles / batch - 0.5 * tokens / batch);
   const double units = (rows / 8 + 0.5 * batch) * kv_heads, few = 5.0 + units * 0.010 + units * mean_keys / 30000;
