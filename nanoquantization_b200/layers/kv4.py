@@ -19,6 +19,7 @@ import torch
 from .. import _lib
 
 DIM, TOKEN = 128, 72
+SPLIT_KEYS = 4096   # decode steps of tables for fewer keys need no scratch
 TILE = 128          # keys of a tile of prompt_attention, which take 512 bytes each per key/value head while it runs
 MOST_SCRATCH = 1 << 30      # for such tiles; more sequences than fit are taken in several goes
 
@@ -117,15 +118,13 @@ def decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.
     lib = _lib.load()
     with _lib.on_device(dev) as stream:
         out = qkv.new_empty((B, num_q_heads * DIM))
-        call = [qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM, positions.data_ptr(),
-                rows.data_ptr(), cache, table.data_ptr(), width, ctx.data_ptr(), out.data_ptr(), B, num_q_heads, DIM ** -0.5 if scale is None else scale, eps, code,
-                None, 0, _lib.cache_status(dev), stream]
-        status = lib.nqb200_kv4_decode_attention(*call)
-        if status == 5:        # a few long sequences, whose clusters' shares need room (asking ahead would cost every other call)
-            need = lib.nqb200_kv4_decode_scratch_bytes(width, cache.block_size, B, num_q_heads, num_kv_heads)
-            scratch = k_cache.new_empty(need)
-            call[18], call[19] = scratch.data_ptr(), need
-            status = lib.nqb200_kv4_decode_attention(*call)
+        # (asked where the answer can be other than 0: a call of a few microseconds is made as often as the host can make it)
+        need = lib.nqb200_kv4_decode_scratch_bytes(width, cache.block_size, B, num_q_heads, num_kv_heads) if width * cache.block_size >= SPLIT_KEYS else 0
+        scratch = k_cache.new_empty(need) if need else None
+        status = lib.nqb200_kv4_decode_attention(qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), cos_sin.numel() // DIM,
+                                                 positions.data_ptr(), rows.data_ptr(), cache, table.data_ptr(), width, ctx.data_ptr(), out.data_ptr(), B,
+                                                 num_q_heads, DIM ** -0.5 if scale is None else scale, eps, code, scratch.data_ptr() if need else None, need,
+                                                 _lib.cache_status(dev), stream)
     _lib.check(status)
     return out
 

@@ -57,6 +57,18 @@ def test_refusals_of_the_attention():
     assert prompt(q=None) == prompt(table=None) == prompt(cu=None) == prompt(out=None) == 4 and prompt(q=P + 8) == prompt(out=P + 8) == 3
 
 
+def test_decode_steps_of_short_tables_need_no_scratch():
+    need = _lib.load().nqb200_kv4_decode_scratch_bytes
+    for block in (16, 48, 256):
+        for batch in (1, 2, 3, 8, 100):
+            for heads, kv_heads in ((1, 1), (8, 1), (32, 8), (64, 8)):
+                width = kv4.SPLIT_KEYS // block
+                assert need(width - (width * block >= kv4.SPLIT_KEYS), block, batch, heads, kv_heads) == 0
+    assert need(16, 256, 1, 8, 1) > 0 and need(1 << 20, 16, 1, 8, 1) > 0
+    for bad in ((0, 16, 1, 8, 1), (16, 0, 1, 8, 1), (16, 256, 0, 8, 1), (16, 256, 1, 9, 2), (16, 256, 1, 8, 0), (1 << 31, 16, 1, 8, 1)):
+        assert need(*bad) == 0
+
+
 def test_which_way_a_prompt_takes():
     name = _lib.load().nqb200_kv4_prompt_kernel_name
     assert name(1, 0, 1, 1, 1, 4, 2) == name(0, 1, 1, 1, 1, 4, 2) == name(1, 1, 1, 1, 1, 4, 3) == name(1, 2, 2, 1, 1, 4, 2) == b"invalid"
