@@ -72,6 +72,33 @@ def test_logits_do_not_depend_on_how_the_tokens_came(dtype):
     assert _rel(want, full) <= 0.35
 
 
+@torch.no_grad()
+def test_prompts_in_portions_beside_whole_ones():
+    m = _model(torch.float16, 6)
+    prompts = [_tokens(n, 70 + n) for n in (300, 9, 120, 64)]
+    whole = _engine(m, num_blocks=80).generate(prompts, 3)
+    for portion in (50, 128, 1):
+        e = _engine(m, num_blocks=80, prefill_portion=portion)
+        got = e.generate(prompts if portion > 1 else prompts[1:2], 3)
+        assert [o[0] for o in got] == [o[0] for o in (whole if portion > 1 else whole[1:2])] and len(e.blocks.free) == 80
+
+
+@torch.no_grad()
+def test_forks_of_a_full_cache_are_refused_and_leave_it_as_it_was():
+    m = _model(torch.float16, 7)
+    e = _engine(m, num_blocks=4)
+    s = Sequence(0, [], 1 << 30)
+    e.extend([(s, _tokens(60, 3), [])])                # four blocks, the last one not full
+    t = e.fork(s)
+    with pytest.raises(RuntimeError, match="cannot hold"):
+        e.extend([(t, [5], [0])])                      # no block is left for a copy
+    assert t.blocks == s.blocks and not e.blocks.copies
+    e.drop(t)
+    assert torch.isfinite(e.extend([(s, [5], [0])])[0]).all() and not e.blocks.shared
+    e.drop(s)
+    assert sorted(e.blocks.free) == [0, 1, 2, 3]
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @torch.no_grad()
 def test_forks_go_on_as_their_sequences_would(bits):
