@@ -239,8 +239,8 @@ int nqb200_kv4_store(const void* qkv, int64_t row_stride, const void* q_weight, 
 int nqb200_kv4_load(const nqb200_kv4* cache, const int64_t* rows, void* k_out, void* v_out, int64_t n, int dtype, int* status, void* stream);
 
 /* nqb200_decode_attention over such a cache: norm, rotation and store of one token per sequence, then attention over ctx[b] keys, the
- * token's own among them (as it is stored).  table [batch, table_width].  ctx[b] = 0 is a row without a sequence: zeros, and nothing of
- * its table, row and position is read.  rows[b] < 0: the token is attended to and not stored. */
+ * token's own among them (as it is stored).  table [batch, table_width], with room for at most 2^31 - 257 keys.  ctx[b] = 0 is a row
+ * without a sequence: zeros, and nothing of its table, row and position is read.  rows[b] < 0: the token is attended to and not stored. */
 int nqb200_kv4_decode_attention(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight, const float* cos_sin,
                                 int64_t max_positions, const int64_t* positions, const int64_t* rows, const nqb200_kv4* cache,
                                 const int32_t* table, int64_t table_width, const int32_t* ctx, void* out, int64_t batch,

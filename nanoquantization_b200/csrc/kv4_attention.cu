@@ -711,7 +711,8 @@ size_t scratch_bytes_of(int64_t batch, int64_t tokens, int64_t max_len, int64_t 
   return s.parts > 1 ? (size_t)(tokens * heads * s.parts * kShare) * sizeof(float) : 0;
 }
 bool heads_fit(int64_t heads, int64_t kv_heads) { return kv_heads > 0 && kv_heads <= 4096 && heads > 0 && heads <= 65535 && heads % kv_heads == 0; }
-bool table_fits(int64_t width, int64_t block) { return width > 0 && block > 0 && width <= INT32_MAX / block; }
+// (keys are numbered in 32 bits, up to the end of the last tile)
+bool table_fits(int64_t width, int64_t block) { return width > 0 && block > 0 && width <= (INT32_MAX - 256) / block; }
 
 }  // namespace
 }  // namespace nqb200

@@ -57,6 +57,17 @@ def test_refusals_of_the_attention():
     assert prompt(q=None) == prompt(table=None) == prompt(cu=None) == prompt(out=None) == 4 and prompt(q=P + 8) == prompt(out=P + 8) == 3
 
 
+def test_tables_whose_last_tile_would_pass_31_bits_are_refused():
+    lib = _lib.load()
+    for block in (16, 48, 256):
+        most = (2**31 - 1 - 256) // block
+        for width in (most + 1, (2**31 - 1) // block):
+            assert lib.nqb200_kv4_decode_attention(P, 1024, P, P, P, 10, P, P, _c(block=block), P, width, P, P, 1, 4, 0.1, 1e-6, 0, P, 1 << 40, None, None) == 1
+            assert lib.nqb200_kv4_prompt_attention(P, 512, _c(block=block), P, width, P, P, P, 1, 4, 4, 4, 1, 4, 0.1, 0, P, 1 << 40, None, None) == 1
+            assert lib.nqb200_kv4_decode_scratch_bytes(width, block, 1, 4, 2) == 0
+        assert lib.nqb200_kv4_decode_scratch_bytes(most, block, 1, 4, 2) > 0
+
+
 def test_decode_steps_of_short_tables_need_no_scratch():
     need = _lib.load().nqb200_kv4_decode_scratch_bytes
     for block in (16, 48, 256):
