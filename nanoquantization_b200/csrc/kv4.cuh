@@ -171,10 +171,10 @@ template <bool BF16> __device__ __forceinline__ void quantise(const Half& hx, co
   words = make_uint2(word[0], word[1]);
 }
 
-// A level as a 16-bit number.  The highest one may lie beyond the type's largest number by the scale's rounding: it is that number.
-template <bool BF16> __device__ __forceinline__ uint16_t level(float n, float scale, float offset) {
+// A level within the type's numbers: the highest one may lie beyond the largest by the scale's rounding, and is that number then.
+template <bool BF16> __device__ __forceinline__ float level(float n, float scale, float offset) {
   constexpr float kTop = BF16 ? 3.3895313892515355e38f : 65504.f;
-  return float_to_raw16<BF16>(min_nan(max_nan(fmaf(n, scale, offset), -kTop), kTop));
+  return min_nan(max_nan(fmaf(n, scale, offset), -kTop), kTop);
 }
 
 __device__ __forceinline__ float nibble(uint32_t word, int i) { return (float)((word >> (4 * i)) & 15u); }

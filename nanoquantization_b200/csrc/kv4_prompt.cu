@@ -3,8 +3,10 @@
 // Two launches.  The first takes the visible pages apart, once, into tiles of 128 keys and 128 values in float16, each 32 KB as the tensor
 // cores want it in shared memory (blocks of 64 dimensions, rows of 128 bytes, swizzled), so that the second fetches a tile with one bulk copy
 // and needs no tensor map.  float16 whatever the model's type: keys, values and weights in bfloat16 cost twice the error of the
-// result's own rounding (a prompt of 8000 tokens: 0.0031 in the 2-norm, 0.0017 so).  A tile whose numbers float16 would not hold well is in units of a
-// power of two, and so is a query.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the
+// result's own rounding (a prompt of 8000 tokens: 0.0031 in the 2-norm, 0.0017 so).  A bfloat16 model may have numbers that float16 would not
+// hold well.  A tile of keys is then in units of a power of two, and so is a query.  A tile of values has no unit, since weights times units would
+// lose what float16 does not hold of the product: it is in bfloat16 instead, and its weights are (values_fit).  So the precision of a row depends
+// on what it sees.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the
 // first of those stands is noted, and the rows that see it get NaN at the end, and no other (a weight of 0 times NaN would be one).
 //
 // In the second a CTA takes 256 rows of a key/value head, as two tiles of 128: a row is a query head of a token, the heads of a group beside
@@ -12,15 +14,15 @@
 //   warp 0        copies: two-stage rings of K tiles and of V tiles.
 //   warps 1, 2    one lane of each issues tcgen05.mma for a query tile: S = Q K^T of a half (both operands in shared memory)
 //                 and O += P V (P in tensor memory, V in shared memory as it lies there: the operand's rows are keys).
-//   warp 3        looks for tiles in other units than 1, and for values that are not finite.
+//   warp 3        looks for tiles of keys in other units than 1, tiles of values in bfloat16, and values that are not finite.
 //   warps 4-19    softmax: four warps for each half of each query tile, a thread per row and half.
 // Tensor memory holds S of both tiles (two halves of 64 columns each) and O of both; P overwrites the first half of its own S.  So four
 // chains S -> weights -> O += P V -> next S run beside each other.
 //
-// The weights are 2^(score - m).  m is the largest score of the row's first tile and follows the largest score when it falls behind by more than
-// kLag in log2 units; O and the sums are then rescaled, which hardly ever happens.  A half finds out by itself that its scores ask
-// for no move, from their largest magnitude; that the other half has not moved it learns from what that one hands on, in the order of the
-// products.  The sum that a row is divided by takes the weights in float, before the product's rounding to 16 bits.
+// The weights are 2^(score - m + 8), so that float16 holds them fully down to 2^-22 of a row's largest; none is above 2^15.  m is the largest
+// score of the row's first tile and follows the largest score when it falls behind by more than kLag in log2 units; O and the sums are then
+// rescaled, which hardly ever happens.  A half finds out by itself that its scores ask for no move, from their largest magnitude; that the
+// other half has not moved it learns from what that one hands on, in the order of the products.  The sum that a row is divided by takes the weights in float, before the product's rounding to 16 bits.
 //
 // One prompt of 8000 tokens, 32 heads over 8: 485 us (1.08 PFLOP/s of visible pairs, 0.66 of the measured peak; 560 back to back under the power
 // cap), of them about 10 for the first launch; 500 tokens behind 12000, 64 heads over 8, 211 (0.95 PFLOP/s: 128 CTAs on 148 SMs); 1000 tokens 33.
@@ -44,23 +46,32 @@ using namespace att;
 constexpr int kTileKeys = 128, kThreads = 640, kRows = 256;
 constexpr uint32_t kTileBytes = kTileKeys * kDim * 2, kBox = kTileKeys * 128;       // of K or V; of a block of 64 dimensions
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
-constexpr float kLog2e = 1.4426950408889634f, kLag = 7.f;
+constexpr float kLog2e = 1.4426950408889634f, kLag = 7.f, kRoom = 8.f;      // 2^(kLag + kRoom) is a number of float16
 constexpr int kNone = 0x7FFFFFFF;
 
 struct alignas(16) TileInfo {
   int bad[2];            // the tile's first key whose value is not finite in dimensions 0..63, in 64..127, or kNone
-  float k, v;            // units of the tile's keys and values
+  float k;               // unit of the tile's keys
+  int wide;              // 0: values in float16; else in bfloat16, 1 + the binary orders above kMostOrder of the largest
 };
-// The unit of numbers up to `top`: 1 where float16 holds them well, else the power of two that puts `top` between 2^13 and 2^14.
+// The unit of numbers up to `top`: 1 where float16 holds them well (its spacing of 2^-24 below 2^-14 is half of a rounding of 2^-12), else the
+// power of two that puts `top` between 2^13 and 2^14.
 __device__ __forceinline__ float unit_of(float top) {
-  if (top == 0.f || (top >= 0.015625f && top < 32768.f)) return 1.f;
+  if (top == 0.f || (top >= 0.000244140625f && top < 32768.f)) return 1.f;
   const uint32_t e = min(max(__float_as_uint(top) >> 23, 15u), 254u);
   return __uint_as_float((e - 13u) << 23);
 }
+// Whether float16 products hold values up to `top` in a group as well as others have to be: rounded to float16 they are 2^-13 of the group's largest off
+// at most, and a weight that float16 no longer holds (half of its spacing is 2^-33 of the row's largest) takes 2^-21 at most, which is
+// 2^-9 of the smallest group's.
+__device__ __forceinline__ bool values_fit(float top) { return top == 0.f || (top >= 0.000244140625f && top < 4096.f); }
+// Weights times values of more than this many binary orders could leave float's range: such tiles count as higher scores, in the rows' references.
+constexpr int kMostOrder = 75;
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+template <bool BF16> __device__ __forceinline__ uint32_t pack16(float lo, float hi) { return BF16 ? pack_bf16(lo, hi) : pack_half(lo, hi); }
 
 struct Params {
   const uint16_t* q; int64_t q_stride;
@@ -98,7 +109,7 @@ __device__ __forceinline__ int tiles_before(const Params& p, int b) {
 // A tile of 128 rows of a key/value head: 16 lanes a row, lane 2 m + j takes word 2 m + j, 8 dimensions, 16 bytes out.
 template <bool BF16>
 __global__ void __launch_bounds__(512, 3) kv4_expand_kernel(const __grid_constant__ Params p) {
-  __shared__ int s_before, s_bad[2];
+  __shared__ int s_before, s_bad[2], s_unfit;
   __shared__ uint32_t s_top[2];
   grid_launch_dependents();
   grid_dependency_wait();
@@ -111,6 +122,7 @@ __global__ void __launch_bounds__(512, 3) kv4_expand_kernel(const __grid_constan
   const int key0 = tile * kTileKeys;
   if (key0 >= s.keys) return;
   if (threadIdx.x < 2) { s_bad[threadIdx.x] = kNone; s_top[threadIdx.x] = 0u; }
+  if (threadIdx.x == 0) s_unfit = 0;
   if (threadIdx.x < 32) {
     const int before = tiles_before(p, b);
     if (threadIdx.x == 0) s_before = before;
@@ -148,42 +160,50 @@ __global__ void __launch_bounds__(512, 3) kv4_expand_kernel(const __grid_constan
       const float sc = scale_of<BF16>(params[which][i]), off = offset_of<BF16>(params[which][i]), most = max_nan(fabsf(off), fabsf(fmaf(15.f, sc, off)));
       if (there[i] && most < INFINITY) {
         top[which] = fmaxf(top[which], most);
+        if (BF16 && which && !values_fit(most)) s_unfit = 1;
       } else if (there[i] && which) {
         atomicMin(&s_bad[j], key0 + i * 32 + (int)(threadIdx.x >> 4));
       }
     }
   }
+  if (BF16) {                                   // (float16 holds a float16 model's numbers)
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top[which]));
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_top[which], all);
+    for (int which = 0; which < 2; ++which) {
+      const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top[which]));
+      if ((threadIdx.x & 31) == 0) atomicMax(&s_top[which], all);
+    }
   }
   __syncthreads();
-  const float unit[2] = {unit_of(__uint_as_float(s_top[0])), unit_of(__uint_as_float(s_top[1]))};
+  const float unit = BF16 ? unit_of(__uint_as_float(s_top[0])) : 1.f, by = 1.f / unit;      // a power of two
+  const bool wide = BF16 && s_unfit;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const float by = 1.f / unit[which];         // a power of two
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = i * 32 + (threadIdx.x >> 4);
-      const float sc = scale_of<BF16>(params[which][i]) * by, off = offset_of<BF16>(params[which][i]) * by;
+      const float sc = scale_of<BF16>(params[which][i]) * (which ? 1.f : by), off = offset_of<BF16>(params[which][i]) * (which ? 1.f : by);
       const bool zero = !there[i] || (which && !(max_nan(fabsf(off), fabsf(fmaf(15.f, sc, off))) < INFINITY));
       uint32_t out[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = zero ? 0u : pack_half(fmaf(nibble(word[which][i], e), sc, off), fmaf(nibble(word[which][i], e + 4), sc, off));
+      for (int e = 0; e < 4; ++e) {
+        const float lo = nibble(word[which][i], e), hi = nibble(word[which][i], e + 4);
+        out[e] = zero ? 0u : BF16 ? pack_half(fmaf(lo, sc, off), fmaf(hi, sc, off)) : pack_half(level<false>(lo, sc, off), level<false>(hi, sc, off));
+      }
+      if (BF16 && which && wide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = zero ? 0u : pack_bf16(level<true>(nibble(word[1][i], e), sc, off), level<true>(nibble(word[1][i], e + 4), sc, off));
+      }
       *reinterpret_cast<uint4*>(dst + which * kTileBytes + j * kBox + r * 128 + ((m ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
-  if (threadIdx.x == 0) p.info[at * p.cache.kv_heads + h] = TileInfo{{s_bad[0], s_bad[1]}, unit[0], unit[1]};
+  if (threadIdx.x == 0) {
+    const int order = (int)(s_top[1] >> 23) - 127;
+    p.info[at * p.cache.kv_heads + h] = TileInfo{{s_bad[0], s_bad[1]}, unit, wide ? 1 + max(order + 1 - kMostOrder, 0) : 0};
+  }
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-template <bool BF16> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if (BF16) return pack_bf16(lo, hi);
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <bool BF16>
@@ -194,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
   __shared__ float s_x[2][2][2][128], s_m[2][2][128];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_i, s_before, s_bad[2], s_special;
-  __shared__ float s_row[kRows], s_unit_v;     // units of the queries; the largest of the values'
+  __shared__ float s_row[kRows];     // units of the queries
   volatile int* s_abort = &s_abort_i;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem_q = smem_raw + (smem - smem_u32(smem_raw));
@@ -319,12 +339,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     const int q = warp - 1;
     const bool el = elect_one();
     const uint32_t idesc_s = umma_idesc(0, 128, kTileKeys / 2);
-    const uint32_t idesc_o = umma_idesc(0, 128, kDim) | (1u << 16);   // B's rows run along k
+    const uint32_t idesc_o = umma_idesc(0, 128, kDim) | (1u << 16), idesc_w = umma_idesc(1, 128, kDim) | (1u << 16);   // B's rows run along k
     const uint64_t dq = umma_smem_desc_sw128(smem + q * kQBytes), dk = umma_smem_desc_sw128(smem + kOffK), dv = smem_desc_mn(smem + kOffV, kBox);
     const uint32_t k_hi = (uint32_t)(dq >> 32), v_hi = (uint32_t)(dv >> 32), q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, v_lo = (uint32_t)dv;
     const uint32_t tS = tmem + kColS + q * 128, tO = tmem + kColO + q * 128;
     const int mine = nq[q], others = nq[q ^ 1];
-    bool ok = mine > 0;
+    bool ok = mine > 0, special = false;
     for (int j = 0; ok && j <= mine; ++j) {
       const int i = j - 1, s = j & 1, so = s ^ 1;
 #pragma unroll
@@ -334,10 +354,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
           ok = ok && poll_bar_warp(&bar_p[q][half], so, s_abort, p.status);
           if (!ok) break;
           tc_fence_after();
+          if (BF16 && i == 0) special = s_special;      // (the weights were made behind warp 3's report)
+          const bool wide = special && p.info[(int64_t)(tile0 + i) * p.cache.kv_heads + blockIdx.y].wide != 0;
           if (el) {
 #pragma unroll
             for (int ks = 0; ks < kTileKeys / 32; ++ks)
-              umma_ts_lohi(tO, tS + half * 64 + ks * 8, v_lo + so * (kTileBytes >> 4) + half * (8192 >> 4) + ks * (2048 >> 4), v_hi, idesc_o,
+              umma_ts_lohi(tO, tS + half * 64 + ks * 8, v_lo + so * (kTileBytes >> 4) + half * (8192 >> 4) + ks * (2048 >> 4), v_hi, wide ? idesc_w : idesc_o,
                            (i > 0 || half > 0 || ks > 0) ? 1u : 0u);
             umma_commit(smem_u32(j == mine && half == 1 ? &bar_o[q] : &bar_pv[q][half]));
             if (half == 1) {
@@ -369,25 +391,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
     if (el) umma_commit(smem_u32(&bar_drain));
     mbar_wait(smem_u32(&bar_drain), 0);
   } else if (warp == 3) {
-    // ------------------------------------------------ units, and values that are not finite
+    // ------------------------------------------------ units and types of tiles, and values that are not finite
     int low[2] = {kNone, kNone};
-    uint32_t unit_v = 0u;
     bool special = false;
     for (int j = lane; j < n_tiles; j += 32) {
       const TileInfo v = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y];
       low[0] = min(low[0], v.bad[0]);
       low[1] = min(low[1], v.bad[1]);
-      unit_v = max(unit_v, __float_as_uint(v.v));
-      special = special || v.k != 1.f || v.v != 1.f;
+      special = special || v.k != 1.f || v.wide != 0;
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g) low[g] = __reduce_min_sync(0xFFFFFFFFu, low[g]);
-    unit_v = __reduce_max_sync(0xFFFFFFFFu, unit_v);
     special = __any_sync(0xFFFFFFFFu, special);
     if (lane == 0) {
       s_bad[0] = low[0];
       s_bad[1] = low[1];
-      s_unit_v = __uint_as_float(unit_v);
       s_special = special;
       mbar_arrive(smem_u32(&bar_bad));
     }
@@ -439,119 +457,128 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       return j < 2 || take(j - 1);
     };
     bool ok = wait_bar_warp(&bar_bad, 0, s_abort, p.status);
-    // the first position of the warp; with tiles in other units every tile takes the general way
-    const int wfirst = s_special ? -1 : pos_of(i - lane);
-    for (int j = 0; ok && j < nq[q]; ++j) {
-      const bool joint = j == 0;
-      ok = catch_up(j) && wait_bar_warp(&bar_s[q][half], j & 1, s_abort, p.status);
-      if (!ok) break;
-      tc_fence_after();
-      const int key0 = kstart + j * kTileKeys + half * 64;
-      const bool masked = key0 + 63 > wfirst;     // for any row of the warp
-      float factor = row_factor;
-      if (masked && s_special) factor *= p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].k;
-      uint32_t r[2][32];     // the row's scores, all of this half
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld32(tS + c * 32, r[c]);
-      tc_wait_ld();
-      // what the row does not see: scores below all others
-      const int left = pos - key0;
-      auto mask = [&](uint32_t (&v)[32], int from) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = from + e <= left ? v[e] : 0xFF800000u;
-      };
-      float mx = -INFINITY;  // where it is asked for, the largest score
-      bool look = joint || masked;
-      if (masked) {
-        mask(r[0], 0);
-        mask(r[1], 32);
-      } else if (!joint) {   // a half finds out from the largest magnitude that nothing moves
-        float hi[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3_abs(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-        look = !__all_sync(0xFFFFFFFFu, fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])) * factor <= m + kLag);
-      }
-      const float lag = m + kLag;
-      if (look) {
-        float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-        mx = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
-        if (joint) {
-          float mo;
-          if (!(ok = exchange(mx, mo))) break;
-          mx = fmaxf(mx, mo);
-        }
-        mx = mx == -INFINITY ? mx : mx * factor;
-      }
-      const bool move = mx > lag;      // also from -inf
-      if (!joint) pass(move ? mx : m);
-      if (j == 0) {
-        m = mx;
-      } else if (__any_sync(0xFFFFFFFFu, move)) {
-        const float f = move ? ex2(m - mx) : 1.f;
-        lsum = mul2(lsum, pair2(f, f));
-        m = move ? mx : m;
-        // O has the products of all halves before this one, and no other until this one's weights are reported
-        if (!(ok = wait_bar_warp(&bar_pv[q][half ^ 1], (j - 1 + half) & 1, s_abort, p.status))) break;
+    const int wfirst = pos_of(i - lane);        // the first position of the warp
+    // SPECIAL: some tile has keys in units other than 1 or values in bfloat16
+    const auto tiles = [&](auto special) {
+      constexpr bool SPECIAL = decltype(special)::value;
+      for (int j = 0; ok && j < nq[q]; ++j) {
+        const bool joint = j == 0;
+        ok = catch_up(j) && wait_bar_warp(&bar_s[q][half], j & 1, s_abort, p.status);
+        if (!ok) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < kDim / 32; ++c) {
-          tmem_ld32(tO + c * 32, r[0]);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) r[0][e] = __float_as_uint(__uint_as_float(r[0][e]) * f);
-          tmem_st32(tO + c * 32, r[0]);
+        const int key0 = kstart + j * kTileKeys + half * 64;
+        const bool masked = key0 + 63 > wfirst;     // for any row of the warp
+        float factor = row_factor;
+        int wide = 0;
+        if (SPECIAL) {
+          const TileInfo t = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y];
+          factor = fmaxf(factor * t.k, 1e-37f);
+          wide = t.wide;
         }
-        tc_wait_st();
-        tmem_ld32(tS, r[0]);      // the scores again
+        uint32_t r[2][32];     // the row's scores, all of this half
+  #pragma unroll
+        for (int c = 0; c < 2; ++c) tmem_ld32(tS + c * 32, r[c]);
         tc_wait_ld();
-        if (masked) mask(r[0], 0);
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
-      const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(factor, factor);
-      if (!masked || !s_special) {
-        uint64_t ls[2] = {lsum, 0};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            unpair2(fma2(pair2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), k1, nm2), x0, x1);
-            x0 = ex2(x0);
-            x1 = ex2(x1);
-            w[e] = pack_half(x0, x1);
-            ls[e & 1] = add2(ls[e & 1], pair2(x0, x1));
-          }
-          tmem_st16(tS + c * 16, w);
+        // what the row does not see: scores below all others
+        const int left = pos - key0;
+        auto mask = [&](uint32_t (&v)[32], int from) {
+  #pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = from + e <= left ? v[e] : 0xFF800000u;
+        };
+        float mx = -INFINITY;  // where it is asked for, the largest score
+        bool look = joint || masked;
+        if (masked) {
+          mask(r[0], 0);
+          mask(r[1], 32);
+        } else if (!joint) {   // a half finds out from the largest magnitude that nothing moves
+          float hi[4] = {0.f, 0.f, 0.f, 0.f};
+  #pragma unroll
+          for (int c = 0; c < 2; ++c)
+  #pragma unroll
+            for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3_abs(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+          look = (SPECIAL && wide > 1) || !__all_sync(0xFFFFFFFFu, fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])) * factor <= m + kLag);
         }
-        lsum = add2(ls[0], ls[1]);
-      } else {
-        // from tensor memory again, a piece at a time: compact code for sequences with tiles in other units
-        const float by = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y].v / s_unit_v;      // of the tile's weights in the product
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[16], w[8];
-          tmem_ld_32x32b_x16(tS + c * 16, v);
+        const float lag = m + kLag;
+        if (look) {
+          float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  #pragma unroll
+          for (int c = 0; c < 2; ++c)
+  #pragma unroll
+            for (int e = 0; e < 32; e += 2) hi[(e >> 1) & 3] = max3(hi[(e >> 1) & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+          mx = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]));
+          if (joint) {
+            float mo;
+            if (!(ok = exchange(mx, mo))) break;
+            mx = fmaxf(mx, mo);
+          }
+          mx = mx == -INFINITY ? mx : mx * factor;
+          if (SPECIAL && wide > 1) mx += (float)(wide - 1);
+        }
+        const bool move = mx > lag;      // also from -inf
+        if (!joint) pass(move ? mx : m);
+        if (j == 0) {
+          m = mx;
+        } else if (__any_sync(0xFFFFFFFFu, move)) {
+          const float f = move ? ex2(m - mx) : 1.f;
+          lsum = mul2(lsum, pair2(f, f));
+          m = move ? mx : m;
+          // O has the products of all halves before this one, and no other until this one's weights are reported
+          if (!(ok = wait_bar_warp(&bar_pv[q][half ^ 1], (j - 1 + half) & 1, s_abort, p.status))) break;
+          tc_fence_after();
+  #pragma unroll 1
+          for (int c = 0; c < kDim / 32; ++c) {
+            tmem_ld32(tO + c * 32, r[0]);
+            tc_wait_ld();
+  #pragma unroll
+            for (int e = 0; e < 32; ++e) r[0][e] = __float_as_uint(__uint_as_float(r[0][e]) * f);
+            tmem_st32(tO + c * 32, r[0]);
+          }
+          tc_wait_st();
+          tmem_ld32(tS, r[0]);      // the scores again
           tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float x[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) x[u] = key0 + c * 16 + 2 * e + u <= pos ? ex2(fmaf(__uint_as_float(v[2 * e + u]), factor, -mu)) : 0.f;
-            w[e] = pack_half(x[0] * by, x[1] * by);
-            lsum = add2(lsum, pair2(x[0], x[1]));
-          }
-          tmem_st8(tS + c * 8, w);      // lies behind what has been read of S
+          if (masked) mask(r[0], 0);
         }
+        const float mu = (m == -INFINITY ? 0.f : m) - kRoom;
+        const uint64_t nm2 = pair2(-mu, -mu), k1 = pair2(factor, factor);
+        if (!SPECIAL || wide == 0) {
+          uint64_t ls[2] = {lsum, 0};
+  #pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t w[16];
+  #pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x0, x1;
+              unpair2(fma2(pair2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), k1, nm2), x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              w[e] = pack_half(x0, x1);
+              ls[e & 1] = add2(ls[e & 1], pair2(x0, x1));
+            }
+            tmem_st16(tS + c * 16, w);
+          }
+          lsum = add2(ls[0], ls[1]);
+        } else {
+          // from tensor memory again, a piece at a time: compact code for tiles whose values are in bfloat16
+  #pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[16], w[8];
+            tmem_ld_32x32b_x16(tS + c * 16, v);
+            tc_wait_ld();
+  #pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float x[2];
+  #pragma unroll
+              for (int u = 0; u < 2; ++u) x[u] = key0 + c * 16 + 2 * e + u <= pos ? ex2(fmaf(__uint_as_float(v[2 * e + u]), factor, -mu)) : 0.f;
+              w[e] = pack_bf16(x[0], x[1]);
+              lsum = add2(lsum, pair2(x[0], x[1]));
+            }
+            tmem_st8(tS + c * 8, w);      // lies behind what has been read of S
+          }
+        }
+        done();
       }
-      done();
-    }
+    };
+    if (!BF16 || !s_special) tiles(std::false_type()); else tiles(std::true_type());
     // Rows go out through shared memory (the queries' place, which no product reads any more), so that a store's lanes write to four lines and
     // not to 32: a warp stages its 32 rows x 128 bytes, piece c of row r at c ^ r mod 8.
     const int R = p.heads / p.cache.kv_heads, at = min(i, span_of(p, blockIdx.z).n * R - 1);      // (again, rather than in registers until here)
@@ -585,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         tc_fence_after();
         // dimensions 64 half ..: NaN where a value that the row sees is none
         const float poison = s_bad[half] <= pos ? __int_as_float(0x7FC00000) : 0.f;
-        const float f = shares ? s_unit_v : s_unit_v / l;
+        const float f = shares ? 1.f : 1.f / l;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t r[32];

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Cache c, const int64_t* r
     const float s = scale_of<BF16>(p), m = offset_of<BF16>(p);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      out[e] = (uint32_t)level<BF16>(nibble(word, e), s, m) | ((uint32_t)level<BF16>(nibble(word, e + 4), s, m) << 16);
+      out[e] = (uint32_t)float_to_raw16<BF16>(level<BF16>(nibble(word, e), s, m)) | ((uint32_t)float_to_raw16<BF16>(level<BF16>(nibble(word, e + 4), s, m)) << 16);
   } else if (row >= 0 && lane == 0) {
     report(status, NQB200_ERR_BAD_INDEX);
   }
