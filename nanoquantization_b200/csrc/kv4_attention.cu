@@ -14,8 +14,9 @@
 //            power of two of its own.
 //   values   n - 8 by a packed operation more: over thousands of keys a sum with 1024 in it loses what the tensor cores cut off it (1500 keys:
 //            0.0022 off), and so does, less, one of numbers above 0.  The weight times the value's scale goes into the product, a version for each
-//            of the two groups, rounded to float16 once; scales are taken relative to the largest that the warp has seen, so that
-//            any type's values keep their bits.  What the level 8 stands for is summed in float.
+//            of the two groups, rounded to float16 once; a column's products are relative to the largest that it has had, a power of two, so that what
+//            is small in float16 is small beside that, in any type.  (Relative to the largest scale alone, a key of large values and no weight
+//            took the others' bits.)  What the level 8 stands for is summed in float.
 //   order    a lane owns 16 neighbouring bytes of a key and 8 of a value, which one load fetches; which dimension is which row of a
 //            product follows from that, as the layout of a row was chosen.
 //
@@ -40,7 +41,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32, kCols = 8;
 constexpr int kStage = kTile * 2 * kToken;                    // keys, values, parameters of keys, parameters of values
 constexpr int kOffV = kTile * kData, kOffKP = 2 * kTile * kData, kOffVP = kOffKP + kTile * kParams;
 constexpr int kOS = kDim + 4;                                 // floats of a column's partial sums
-constexpr float kLog2e = 1.4426950408889634f, kLag = 8.f;
+constexpr float kLog2e = 1.4426950408889634f, kLag = 8.f, kAhead = 64.f;      // 2^kLag kAhead is a number of float16
 
 struct Args {
   const uint16_t* q; int64_t stride;              // queries, or the projections of a decode step
@@ -90,6 +91,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // Nibbles I and I + 4 of a word, as pairs of float16: 1024 + n for even I, 1024 + 16 n for odd I.  `magic` is a pair of 1024 in a register:
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) O[i][e] = 0.f;
-  float top_scale = 0.f, inv_scale = 0.f;          // what the values' scales are relative to, a power of two, and its reciprocal
+  float inv[2] = {power_of_two(126), power_of_two(126)};       // the reciprocals of the columns' units of weight times scale, powers of two
 
   // row i of a product's 16 keys is key i ^ bit 1 of i
   const int key_g = g ^ ((g >> 1) & 1), kv0 = (2 * t4) ^ (t4 & 1), kv1 = (2 * t4 + 1) ^ (t4 & 1);
@@ -421,60 +423,69 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
 #pragma unroll
       for (int r = 0; r < 2; ++r) s_top = max3(s_top, scale_of<BF16>(vp[u][r].x), scale_of<BF16>(vp[u][r].y));      // (a NaN is passed over)
     // The first tile sets the reference.  (What a column sees is a beginning of the keys: one that sees nothing of the first tile sees nothing at all.)
-    if (first || __any_sync(0xFFFFFFFFu, top[0] > kLag || top[1] > kLag || s_top > top_scale)) {
+    if (first || __any_sync(0xFFFFFFFFu, top[0] > kLag || top[1] > kLag || s_top * fmaxf(inv[0], inv[1]) > kAhead)) {
+      float most[2] = {-INFINITY, -INFINITY};      // log2 of the tile's largest weight times scale, up to one above it
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s = fmaxf(fmaxf(scale_of<BF16>(vp[u][r].x), scale_of<BF16>(vp[u][r].y)), 0.f), order = (float)((int)(__float_as_uint(s) >> 23) - 126);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) most[h] = fmaxf(most[h], x[u][2 * r + h] + order);
+        }
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
-        top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
-        top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], o));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], o));
+          most[h] = fmaxf(most[h], __shfl_xor_sync(0xFFFFFFFFu, most[h], o));
+        }
       }
-      float far[2], same = 1.f;                    // what the sums so far are multiplied by
+      float far[2];                                // what the sums so far are multiplied by
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float by = first ? (top[h] == -INFINITY ? 0.f : top[h]) : fmaxf(top[h], 0.f);
-        far[h] = first ? 0.f : exp2_fast(-by);
+        const float by = first ? (top[h] == -INFINITY ? 0.f : top[h]) : fmaxf(top[h], 0.f), f = first ? 0.f : exp2_fast(-by);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           x[u][h] -= by;
           x[u][2 + h] -= by;
         }
         ref[h] += by;
-        l[h] *= far[h];
-        L[0][h] *= far[h];
-        L[1][h] *= far[h];
-      }
-      const uint32_t s_all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(s_top));
-      if (__uint_as_float(s_all) > top_scale) {    // to twice the next power of two
-        const float n = __uint_as_float(min((s_all & 0x7F800000u) + 0x01000000u, 0x7E000000u));
-        same = top_scale / n;
-        top_scale = n;
-        inv_scale = 1.f / n;
+        l[h] *= f;
+        L[0][h] *= f;
+        L[1][h] *= f;
+        // the unit: from 2^-110 to 2^125, no less than what the sums so far ask for
+        const int before = 127 - (int)(__float_as_uint(inv[h]) >> 23);
+        const int order = (int)ceilf(fminf(fmaxf((first ? most[h] : fmaxf(most[h], (float)before)) - by, -110.f), 125.f));
+        inv[h] = power_of_two(-order);
+        far[h] = first ? 0.f : exp2_fast((float)(before - order) - by);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) O[i][e] *= far[e & 1] * same;
+        for (int e = 0; e < 4; ++e) O[i][e] *= far[e & 1];
     }
     uint32_t w[2][2][2];                           // [16 keys][half][rows of 8]: weights as the second operand
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float p[2];
+        float p[2], q[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) { p[h] = exp2_fast(x[u][2 * r + h]); l[h] += p[h]; }
+        for (int h = 0; h < 2; ++h) { p[h] = exp2_fast(x[u][2 * r + h]); q[h] = p[h] * inv[h]; l[h] += p[h]; }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t par = half ? vp[u][r].y : vp[u][r].x;
-          const float full = scale_of<BF16>(par), s = full * inv_scale, o = fmaf(8.f, full, offset_of<BF16>(par));
+          const float s = scale_of<BF16>(par), o = fmaf(8.f, s, offset_of<BF16>(par));
           // a key that a column does not see has no part in it, even where its value is not a number
           if (EDGE) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) L[half][h] = seen(u, 2 * r + h) ? fmaf(p[h], o, L[half][h]) : L[half][h];
-            w[u][half][r] = transpose8(pack2(seen(u, 2 * r) ? p[0] * s : 0.f, seen(u, 2 * r + 1) ? p[1] * s : 0.f));
+            w[u][half][r] = transpose8(pack2(seen(u, 2 * r) ? q[0] * s : 0.f, seen(u, 2 * r + 1) ? q[1] * s : 0.f));
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) L[half][h] = fmaf(p[h], o, L[half][h]);
-            w[u][half][r] = transpose8(pack2(p[0] * s, p[1] * s));
+            w[u][half][r] = transpose8(pack2(q[0] * s, q[1] * s));
           }
         }
       }
@@ -526,13 +537,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
       L[1][h] += __shfl_xor_sync(0xFFFFFFFFu, L[1][h], o);
     }
   }
+  const float unit_v[2] = {1.f / inv[0], 1.f / inv[1]};
   float* po = reinterpret_cast<float*>(ring);      // [column][kOS]
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int half = i >> 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float2 v = make_float2(fmaf(O[i][h], top_scale, L[half][h]), fmaf(O[i][2 + h], top_scale, L[half][h]));
+      const float2 v = make_float2(fmaf(O[i][h], unit_v[h], L[half][h]), fmaf(O[i][2 + h], unit_v[h], L[half][h]));
       *reinterpret_cast<float2*>(po + (2 * t4 + h) * kOS + 64 * half + 8 * g + 2 * (i & 3)) = v;
     }
   }

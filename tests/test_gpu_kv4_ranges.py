@@ -84,7 +84,8 @@ def _queries(n, heads, dtype, g, far):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("what", VALUES)
-@pytest.mark.parametrize("n,start,kv_heads,heads,way", [(500, 500, 4, 16, b"tiles_tcgen05"), (64, 6000, 2, 32, b"tiles_tcgen05"), (900, 0, 8, 32, b"tiles_tcgen05")])
+@pytest.mark.parametrize("n,start,kv_heads,heads,way", [(500, 500, 4, 16, b"tiles_tcgen05"), (64, 6000, 2, 32, b"tiles_tcgen05"), (900, 0, 8, 32, b"tiles_tcgen05"),
+                                                        (5, 900, 2, 8, b"rows"), (40, 500, 1, 3, b"rows")])
 @torch.no_grad()
 def test_prompt_values(n, start, kv_heads, heads, way, what, dtype):
     from nanoquantization_b200 import _lib
@@ -101,6 +102,30 @@ def test_prompt_values(n, start, kv_heads, heads, way, what, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", VALUES)
+@pytest.mark.parametrize("total,kv_heads,heads", [(1000, 2, 8), (5000, 1, 8), (300, 8, 16)])
+@torch.no_grad()
+def test_decode_values(total, kv_heads, heads, what, dtype):
+    from nanoquantization_b200.layers import kv4
+    block = 64
+    sizes, heavy = _sizes(what, total, dtype)
+    kc, vc, table, rows, g = _filled(total, kv_heads, block, dtype, sizes, heavy)
+    qkv = torch.randn(1, heads + 2 * kv_heads, D, generator=g, device=DEV)
+    qkv[:, :heads, 64:] = 2.25
+    qkv[:, heads:heads + kv_heads, 64:] = 1.0
+    qkv[:, heads + kv_heads:] = qkv[:, heads + kv_heads:].clamp(-1, 1) * sizes[-1].float()
+    qkv = qkv.flatten(1).to(dtype)
+    w, first = torch.ones(D, device=DEV).to(dtype), torch.zeros(1, dtype=torch.int64, device=DEV)
+    cs = ref.angles(2, DEV)                            # position 0 turns nothing
+    scale = 0.6 if "start without" in what else 0.15   # of queries of 1.3 in the second half, 12.4 or 50 between the keys' scores
+    got = kv4.decode_attention(qkv, w, w, cs, first, heads, kv_heads, 1e-6, kc, vc, table, torch.tensor([total], dtype=torch.int32, device=DEV),
+                               torch.tensor(rows[-1:], device=DEV), scale=scale)
+    k, v = (ref.rows_of(c, rows, block, dtype) for c in (kc, vc))
+    q = ref.norm_rope(qkv.double().view(1, -1, D)[:, :heads], w, cs, first)
+    _each_close(got.view(1, heads, D), ref.attend(q, k, v, total - 1, scale), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("size", [0.0155, 1e-3, "first", "last"])
 @pytest.mark.parametrize("n,start,kv_heads,heads", [(500, 500, 4, 16), (64, 6000, 2, 32)])
 @torch.no_grad()
@@ -114,6 +139,25 @@ def test_prompt_keys(n, start, kv_heads, heads, size, dtype):
     key_size = {"first": torch.where(j < 128, 0.017, 0.0155), "last": torch.where(j >= total - 128, 0.017, 0.0155)}.get(size, torch.full((total,), 0.0155 if isinstance(size, str) else size, device=DEV)).double()
     kc, vc, table, rows, g = _filled(total, kv_heads, block, dtype, torch.ones(total, device=DEV, dtype=torch.float64), None, key_size)
     q = (torch.randn(n, heads, D, generator=g, device=DEV) * float(2 / key_size.max())).to(dtype)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    got = kv4.prompt_attention(q.flatten(1), heads, kc, vc, table, i32(0, n), i32(start), [n], [start])
+    k, v = (ref.rows_of(c, rows, block, dtype) for c in (kc, vc))
+    _each_close(got.view(n, heads, D), ref.attend(q.double(), k, v, start), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [-40.0, 40.0])
+@pytest.mark.parametrize("n,start,kv_heads,heads", [(500, 500, 4, 16), (64, 6000, 2, 32), (5, 900, 2, 8)])
+@torch.no_grad()
+def test_scores_far_from_zero(n, start, kv_heads, heads, shift, dtype):
+    """All scores 226 below or above zero, which moves no weight: 326 in log2 units, beyond float's own range as a power."""
+    from nanoquantization_b200.layers import kv4
+    total, block = n + start, 64
+    sizes, heavy = _sizes("all below 1/64", total, dtype)
+    kc, vc, table, rows, g = _filled(total, kv_heads, block, dtype, sizes, heavy)
+    q = torch.randn(n, heads, D, generator=g, device=DEV)
+    q[..., 64:] = shift
+    q = q.to(dtype)
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
     got = kv4.prompt_attention(q.flatten(1), heads, kc, vc, table, i32(0, n), i32(start), [n], [start])
     k, v = (ref.rows_of(c, rows, block, dtype) for c in (kc, vc))
