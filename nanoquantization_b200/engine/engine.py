@@ -38,7 +38,7 @@ class Sequence:
     output: list[int] = field(default_factory=list)
     blocks: list[int] = field(default_factory=list)
     prefilled: bool = False
-    carried: list[int] = field(default_factory=list)  # tokens generated before a preemption (now part of the prompt)
+    carried: list[int] = field(default_factory=list)  # tokens generated before a preemption or an extension (now part of the prompt)
     computed: int = 0  # tokens that the cache and the states hold
     slot: Optional[int] = None  # recurrent-state slot
     scheduled: int = 0  # tokens that the scheduler gave it in this step
@@ -49,6 +49,12 @@ class Sequence:
     @property
     def finished(self) -> bool:
         return len(self.output) >= self.max_new_tokens
+
+    def carry_output(self) -> None:
+        """What it has generated becomes part of its prompt, and goes on counting."""
+        self.carried += self.output
+        self.max_new_tokens -= len(self.output)
+        self.prompt, self.output = self.prompt + self.output, []
 
 
 class BlockManager:
@@ -302,9 +308,8 @@ class Scheduler:
             self.release(victim)
             if victim in ready:
                 ready.remove(victim)
-            victim.carried += victim.output
-            victim.max_new_tokens -= len(victim.output)
-            victim.prompt, victim.output, victim.prefilled = victim.prompt + victim.output, [], False
+            victim.carry_output()
+            victim.prefilled = False
             self.waiting.appendleft(victim)
         return "decode", ready
 
@@ -475,17 +480,21 @@ class LLMEngine:
     def extend(self, entries: Seq[tuple[Sequence, Seq[int], Seq[int]]]) -> list[torch.Tensor]:
         """One step on tokens that are given, not chosen: ``(sequence, next tokens, wanted places among them)`` per
         entry; returns the wanted logits, ``[places, vocab]`` each.  Single tokens that continue their sequences
-        take the decode path, anything else the prefill path, as in generation."""
-        batch, counts = [s for s, _, _ in entries], [len(t) for _, t, _ in entries]
+        take the decode path, anything else the prefill path, as in generation.  What of a sequence no step has been through yet
+        (a fork's newest token, or the rest of its prompt) comes ahead of its given tokens."""
+        batch = [s for s, _, _ in entries]
         for s, tokens, _ in entries:
+            if s.output:
+                s.carry_output()
             s.prompt.extend(tokens)
             self._hold(s, len(s))
+        counts = [len(s) - s.computed for s in batch]
         if all(n == 1 and s.computed > 0 for s, n in zip(batch, counts)):
             h = self._decode_hidden(batch)[0]
             return [self.model.logits(h[i:i + 1]) if len(want) else None for i, (_, _, want) in enumerate(entries)]
         rows, o = [np.empty(0, np.int64)], 0
-        for (_, _, want), n in zip(entries, counts):
-            rows.append(o + (np.arange(want.start, want.stop, want.step) if isinstance(want, range) else np.array([int(w) for w in want], np.int64)))
+        for (_, tokens, want), n in zip(entries, counts):
+            rows.append(o + n - len(tokens) + (np.arange(want.start, want.stop, want.step) if isinstance(want, range) else np.array([int(w) for w in want], np.int64)))
             o += n
         h = self._run_portions(batch, counts, np.concatenate(rows))
         out, o = [], 0
@@ -495,8 +504,9 @@ class LLMEngine:
         return out
 
     def fork(self, s: Sequence) -> Sequence:
-        """A sequence that goes on, with ``extend``, from where ``s`` stands, which goes on as well.  They share the blocks of what they have in
-        common; one that writes into a shared block gets a copy of it first.  Recurrent states are copied at once."""
+        """A sequence that goes on, with ``extend``, from where ``s`` stands, which goes on as well: a sequence that was given its tokens, or one
+        that waits or generates.  They share the blocks of what they have in common; one that writes into a shared block gets a copy of it
+        first.  Recurrent states are copied at once."""
         t = Sequence(s.seq_id, list(s.prompt), s.max_new_tokens, list(s.output))
         t.prefilled, t.carried, t.computed = s.prefilled, list(s.carried), s.computed
         if self.layout.recurrent and s.slot is not None:
