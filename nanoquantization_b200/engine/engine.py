@@ -483,11 +483,17 @@ class LLMEngine:
         take the decode path, anything else the prefill path, as in generation.  What of a sequence no step has been through yet
         (a fork's newest token, or the rest of its prompt) comes ahead of its given tokens."""
         batch = [s for s, _, _ in entries]
+        ids = {id(s) for s in batch}
+        if len(ids) < len(batch):
+            raise ValueError("a sequence comes twice in a step")
+        if any(id(s) in ids for q in (self.scheduler.running, self.scheduler.waiting) for s in q):
+            raise ValueError("a sequence that the scheduler runs is extended by forks of it")
+        for s, tokens, _ in entries:
+            self._hold(s, len(s) + len(tokens))
         for s, tokens, _ in entries:
             if s.output:
                 s.carry_output()
             s.prompt.extend(tokens)
-            self._hold(s, len(s))
         counts = [len(s) - s.computed for s in batch]
         if all(n == 1 and s.computed > 0 for s, n in zip(batch, counts)):
             h = self._decode_hidden(batch)[0]

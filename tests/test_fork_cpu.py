@@ -1,7 +1,8 @@
 """Forks go on from where their sequences stand: what a step feeds the model, without a GPU (a forward that notes its inputs)."""
+import pytest
 import torch
 
-from nanoquantization_b200.engine import LLMEngine
+from nanoquantization_b200.engine import LLMEngine, Sequence
 from nanoquantization_b200.models.qwen3_quantized import Qwen3QuantizedForCausalLM
 
 
@@ -77,3 +78,31 @@ def test_no_tokens_are_given_but_one_is_left():
     fed.clear()
     assert engine.extend([(t, [], [])]) == [None]
     assert fed == [(True, [42], [3], [0, 1], None)] and t.computed == len(t) == 4
+
+
+def test_steps_that_are_refused():
+    engine, fed = _engine()
+    engine.add_request([1, 2, 3], 10)
+    with pytest.raises(ValueError, match="the scheduler runs"):
+        engine.extend([(engine.scheduler.waiting[0], [5], [0])])
+    engine.step()
+    s = engine.scheduler.running[0]
+    fed.clear()
+    with pytest.raises(ValueError, match="the scheduler runs"):
+        engine.extend([(s, [5], [0])])
+    t = engine.fork(s)
+    with pytest.raises(ValueError, match="twice"):
+        engine.extend([(t, [5], [0]), (t, [6], [0])])
+    assert not fed and t.prompt == [1, 2, 3] and t.output == [42]
+
+
+def test_a_step_that_the_cache_cannot_hold_leaves_the_tokens_out():
+    engine, fed = _engine(num_blocks=2)
+    s = Sequence(0, [], 1 << 30)
+    engine.extend([(s, [1, 2, 3, 4, 5], [])])
+    with pytest.raises(RuntimeError, match="cannot hold"):
+        engine.extend([(s, [6, 7, 8, 9], [])])
+    assert s.prompt == [1, 2, 3, 4, 5]
+    fed.clear()
+    engine.extend([(s, [6], [0])])
+    assert fed == [(True, [6], [5], [0, 1], None)]
