@@ -83,8 +83,9 @@ def _trace(args) -> int:
             if e["tokens"]:
                 entries.append((seq, e["tokens"], e.get("want") or []))
         logits = [t for t in engine.extend(entries) if t is not None] if entries else []
+        data = torch.cat(logits).float().cpu().numpy().astype("<f4") if logits else None
+        engine._check_device_status()      # nothing of a step that a kernel gave up is written
         if logits:
-            data = torch.cat(logits).float().cpu().numpy().astype("<f4")
             with open(os.path.join(args.out, f"{step['step']}.f32"), "wb") as fh:
                 fh.write(data.tobytes())
         for name in step.get("end") or []:

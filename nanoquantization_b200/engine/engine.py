@@ -481,7 +481,7 @@ class LLMEngine:
         """One step on tokens that are given, not chosen: ``(sequence, next tokens, wanted places among them)`` per
         entry; returns the wanted logits, ``[places, vocab]`` each.  Single tokens that continue their sequences
         take the decode path, anything else the prefill path, as in generation.  What of a sequence no step has been through yet
-        (a fork's newest token, or the rest of its prompt) comes ahead of its given tokens."""
+        (a fork's newest token, or the rest of its prompt) comes ahead of its given tokens.  With a cache of 4 bits the step is waited for."""
         batch = [s for s, _, _ in entries]
         ids = {id(s) for s in batch}
         if len(ids) < len(batch):
@@ -497,7 +497,9 @@ class LLMEngine:
         counts = [len(s) - s.computed for s in batch]
         if all(n == 1 and s.computed > 0 for s, n in zip(batch, counts)):
             h = self._decode_hidden(batch)[0]
-            return [self.model.logits(h[i:i + 1]) if len(want) else None for i, (_, _, want) in enumerate(entries)]
+            out = [self.model.logits(h[i:i + 1]) if len(want) else None for i, (_, _, want) in enumerate(entries)]
+            self._check_cache()
+            return out
         rows, o = [np.empty(0, np.int64)], 0
         for (_, tokens, want), n in zip(entries, counts):
             rows.append(o + n - len(tokens) + (np.arange(want.start, want.stop, want.step) if isinstance(want, range) else np.array([int(w) for w in want], np.int64)))
@@ -507,6 +509,7 @@ class LLMEngine:
         for _, _, want in entries:
             out.append(self.model.logits(h[o:o + len(want)]) if len(want) else None)
             o += len(want)
+        self._check_cache()
         return out
 
     def fork(self, s: Sequence) -> Sequence:
@@ -554,6 +557,12 @@ class LLMEngine:
                 s.output.append(int(t))
                 s.prefilled = True
         return self.scheduler.finish_step(kind, complete)
+
+    def _check_cache(self) -> None:
+        """With a cache of 4 bits, wait for the step and raise if a kernel met a page, row or position outside its buffer or gave up a wait."""
+        if self.cache.bits == 4:
+            from .. import _lib
+            _lib.check_cache_status()
 
     def _check_device_status(self) -> None:
         """After the step's results reached the host: raise if a bounded device-side wait gave up during it
