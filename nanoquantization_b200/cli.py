@@ -72,8 +72,12 @@ def _trace(args) -> int:
             continue
         step = json.loads(line)
         entries = []
+        standing = set(live)
         for e in step["entries"]:      # ahead of the step's tokens
-            if e["id"] not in live and e.get("from") is not None:
+            if e.get("from") is not None:
+                if e["id"] in live or e["from"] not in standing:
+                    print(f'step {step["step"]}: "from" is for the first entry of a request and names one that is live, got {e["from"]!r} for {e["id"]!r}', file=sys.stderr)
+                    return 2
                 build.build_library(build.LIB_PATH)      # of the copies
                 live[e["id"]] = engine.fork(live[e["from"]])
         for e in step["entries"]:

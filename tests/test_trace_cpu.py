@@ -80,3 +80,19 @@ def test_a_bad_index_ends_the_step_that_met_it(n, monkeypatch):
         engine.extend([(s, [9] * n, [0])])
     assert not word.any()
     engine.extend([(s, [1] * n, [0])])
+
+
+def test_requests_that_go_on_from_others(trace, capsys):
+    start = {"entries": [{"id": "a", "tokens": [5, 6]}]}
+    assert trace(start, {"entries": [{"id": "b", "from": "a", "tokens": [7], "want": [0]}, {"id": "a", "tokens": [8]}], "end": ["a"]},
+                 {"entries": [{"id": "c", "from": "b", "tokens": [9]}]}) == 0
+    assert capsys.readouterr().out.split() == ["done", "0", "done", "1", "done", "2"]
+    # a request that is not there, that ended, that starts in the same step; one that lives already, or that the step has forked
+    for step in ({"entries": [{"id": "b", "from": "x", "tokens": [7]}]}, {"entries": [{"id": "a", "from": "a", "tokens": [7]}]},
+                 {"entries": [{"id": "b", "tokens": [7]}, {"id": "c", "from": "b", "tokens": [7]}]},
+                 {"entries": [{"id": "b", "from": "a", "tokens": [7]}, {"id": "c", "from": "b", "tokens": [7]}]},
+                 {"entries": [{"id": "b", "from": "a", "tokens": [7]}, {"id": "b", "from": "a", "tokens": [7]}]}):
+        assert trace(start, step) == 2
+        got = capsys.readouterr()
+        assert got.out.split() == ["done", "0"] and '"from"' in got.err and "step 1" in got.err
+    assert trace({**start, "end": ["a"]}, {"entries": [{"id": "b", "from": "a", "tokens": [7]}]}) == 2
