@@ -21,7 +21,7 @@ from .. import _lib
 DIM, TOKEN = 128, 72
 SPLIT_KEYS = 4096   # decode steps of tables for fewer keys need no scratch
 TILE = 128          # keys of a tile of prompt_attention, which take 512 bytes each per key/value head while it runs
-MOST_SCRATCH = 1 << 30      # for such tiles; more sequences than fit are taken in several goes
+MOST_SCRATCH = 1 << 30      # where they go into tiles, more sequences than fit are taken in several goes (one alone may take more)
 
 
 def new_cache(num_blocks: int, block_size: int, kv_heads: int, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -150,11 +150,12 @@ def prompt_attention(q: torch.Tensor, num_q_heads: int, k_cache: torch.Tensor, v
     max_len, max_ctx, tiles = max(lens, default=0), max(ends, default=0), sum([(e + TILE - 1) // TILE for e in ends])
     out = q.new_empty((T, num_q_heads * DIM))
     scale = DIM ** -0.5 if scale is None else scale
-    room = max(1, MOST_SCRATCH // (TILE * 512 * cache.kv_heads))
     with _lib.on_device(dev) as stream:
-        if tiles <= room:
-            _prompt(q, out, num_q_heads, cache, k_cache, code, table, cu, pos0, B, max_len, max_ctx, tiles, scale, stream)
+        need = _lib.load().nqb200_kv4_prompt_scratch_bytes(B, T, max_len, max_ctx, tiles, num_q_heads, cache.kv_heads)
+        if need <= MOST_SCRATCH or B < 2:
+            _prompt(q, out, num_q_heads, cache, k_cache, code, table, cu, pos0, B, max_len, max_ctx, tiles, scale, need, stream)
             return out
+        room = max(1, MOST_SCRATCH // (TILE * 512 * cache.kv_heads))
         b = o = 0
         while b < B:
             e, t, n = b, 0, 0
@@ -163,17 +164,16 @@ def prompt_attention(q: torch.Tensor, num_q_heads: int, k_cache: torch.Tensor, v
                 n += lens[e]
                 e += 1
             if n:
-                some = range(b, e)
-                _prompt(q[o:o + n], out[o:o + n], num_q_heads, cache, k_cache, code, table[b:e], cu[b:e + 1] - o, pos0[b:e], e - b, max(lens[i] for i in some),
-                        max(lens[i] + starts[i] for i in some if lens[i]), t, scale, stream)
+                max_len, max_ctx = max(lens[b:e]), max(lens[i] + starts[i] for i in range(b, e) if lens[i])
+                need = _lib.load().nqb200_kv4_prompt_scratch_bytes(e - b, n, max_len, max_ctx, t, num_q_heads, cache.kv_heads)
+                _prompt(q[o:o + n], out[o:o + n], num_q_heads, cache, k_cache, code, table[b:e], cu[b:e + 1] - o, pos0[b:e], e - b, max_len, max_ctx, t, scale, need, stream)
             b, o = e, o + n
     return out
 
 
-def _prompt(q, out, num_q_heads, cache, k_cache, code, table, cu, pos0, B, max_len, max_ctx, tiles, scale, stream):
-    lib, T, width = _lib.load(), q.shape[0], table.shape[1]
-    need = lib.nqb200_kv4_prompt_scratch_bytes(B, T, max_len, max_ctx, tiles, num_q_heads, cache.kv_heads)
+def _prompt(q, out, num_q_heads, cache, k_cache, code, table, cu, pos0, B, max_len, max_ctx, tiles, scale, need, stream):
+    T, width = q.shape[0], table.shape[1]
     scratch = k_cache.new_empty(need) if need else None
-    _lib.check(lib.nqb200_kv4_prompt_attention(q.data_ptr(), q.stride(0), cache, table.data_ptr(), width, cu.data_ptr(), pos0.data_ptr(), out.data_ptr(), B, T, max_len,
+    _lib.check(_lib.load().nqb200_kv4_prompt_attention(q.data_ptr(), q.stride(0), cache, table.data_ptr(), width, cu.data_ptr(), pos0.data_ptr(), out.data_ptr(), B, T, max_len,
                                                max_ctx, tiles, num_q_heads, scale, code, scratch.data_ptr() if need else None, need,
                                                _lib.cache_status(q.get_device()), stream))
