@@ -252,7 +252,7 @@ size_t nqb200_kv4_decode_scratch_bytes(int64_t table_width, int64_t block_size, 
 /* Causal attention of several tokens per sequence over the cache, which holds their own keys and values too: tokens cu[b] ..
  * cu[b + 1] - 1 of q [T, q_stride] stand at positions pos0[b] .. of sequence b, and each sees all positions up to its own.  out [T,
  * num_q_heads * 128].  What the host knows of the lengths (a bound each; cu and pos0 say the rest): max_len tokens of a sequence, max_ctx keys
- * of one, and the sum over the sequences of their keys' tiles of 128 (`tiles`).  A sequence beyond them is reported as a bad index.
+ * of one, and the sum over the sequences of their keys' tiles of 128 (`tiles`, 2^24 at most).  A sequence beyond them is reported as a bad index.
  * q_stride a multiple of 8. */
 int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, const nqb200_kv4* cache, const int32_t* table, int64_t table_width,
                                 const int32_t* cu, const int32_t* pos0, void* out, int64_t batch, int64_t T, int64_t max_len,

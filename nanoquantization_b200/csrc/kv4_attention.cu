@@ -773,7 +773,7 @@ static bool prompt_goes_umma(int64_t batch, int64_t T, int64_t max_len, int64_t 
 
 extern "C" size_t nqb200_kv4_prompt_scratch_bytes(int64_t batch, int64_t T, int64_t max_len, int64_t max_ctx, int64_t tiles, int64_t num_q_heads, int64_t kv_heads) {
   if (!heads_fit(num_q_heads, kv_heads) || batch <= 0 || batch > 65535 || T <= 0 || max_len <= 0 || max_len > T || max_ctx < max_len || max_ctx > INT32_MAX - 256 || tiles <= 0 ||
-      tiles > INT32_MAX / 2)
+      tiles > kv4::kMostTiles)
     return 0;
   if (prompt_goes_umma(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads))
     return kv4::prompt_umma_scratch_bytes(batch, T, max_len, max_ctx, tiles, num_q_heads, kv_heads);
@@ -790,7 +790,7 @@ extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, cons
                                            int64_t tiles, int64_t num_q_heads, float scale, int dtype, void* scratch, size_t scratch_bytes, int* status, void* stream) {
   const int rc = check_heads(cache, num_q_heads, table_width, dtype);
   if (rc != NQB200_OK) return rc;
-  if (batch < 0 || batch > 65535 || T < 0 || T > INT32_MAX / num_q_heads || max_len < 0 || (T > 0 && max_len > T) || max_ctx < max_len || max_ctx > INT32_MAX - 256 || tiles < 0 || tiles > INT32_MAX / 2 ||
+  if (batch < 0 || batch > 65535 || T < 0 || T > INT32_MAX / num_q_heads || max_len < 0 || (T > 0 && max_len > T) || max_ctx < max_len || max_ctx > INT32_MAX - 256 || tiles < 0 || tiles > kv4::kMostTiles ||
       q_stride < num_q_heads * kv4::kDim || q_stride % 8 != 0)
     return NQB200_ERR_BAD_SHAPE;
   if (batch == 0 || T == 0) return NQB200_OK;

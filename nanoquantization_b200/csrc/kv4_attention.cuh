@@ -5,6 +5,7 @@
 namespace nqb200 {
 namespace kv4 {
 
+constexpr int kMostTiles = 1 << 24;   // of 128 keys, in a prompt call: a terabyte of scratch
 constexpr int kShare = kDim + 4;      // floats of a row's share of its keys: sums, maximum (log2 units), sum of weights
 
 // out[row] = the sum of the row's shares (64 at most), in their order, over its sum of weights; 0 where there is no key.

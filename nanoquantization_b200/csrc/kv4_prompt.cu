@@ -99,10 +99,11 @@ __device__ __forceinline__ Span span_of(const Params& p, int b) {
   s.keys = s.n > 0 ? (int)min(min((int64_t)s.pos0 + s.n, (int64_t)p.max_ctx), p.width * p.cache.block) : 0;
   return s;
 }
-// Tiles of the sequences before b; by all threads of a warp.
+// Tiles of the sequences before b; by all threads of a warp.  Numbers on the device may add up to more than 31 bits where they are not the host's:
+// a sum stops above kMostTiles, which no scratch has room for.
 __device__ __forceinline__ int tiles_before(const Params& p, int b) {
   int sum = 0;
-  for (int i = threadIdx.x & 31; i < b; i += 32) sum += (span_of(p, i).keys + kTileKeys - 1) / kTileKeys;
+  for (int i = threadIdx.x & 31; i < b; i += 32) sum = min(sum + (span_of(p, i).keys + kTileKeys - 1) / kTileKeys, 2 * kMostTiles);
   return __reduce_add_sync(0xFFFFFFFFu, sum);
 }
 
