@@ -53,7 +53,7 @@ struct Args {
   const int32_t *ctx;                             // decode
   const int32_t *cu, *pos0;                       // several tokens per sequence
   uint16_t* out;
-  int heads, groups, tokens, max_len;             // groups: of kCols columns, per key/value head
+  int heads, groups, tokens, max_len, max_ctx;    // groups: of kCols columns, per key/value head
   float scale, eps;
   float* shares; int parts;                       // a sequence over several clusters (parts > 1): their shares
   int* status;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
   const int kvh = blockIdx.y / a.groups, group = blockIdx.y % a.groups, b = blockIdx.z;
   const int R = a.heads / a.cache.kv_heads;
   const int t_first = DECODE ? b : a.cu[b], n_tokens = DECODE ? 1 : a.cu[b + 1] - t_first;
-  if (!DECODE && n_tokens > 0 && (t_first < 0 || n_tokens > a.tokens - t_first)) {      // not rows of q
+  if (!DECODE && n_tokens != 0 && (t_first < 0 || n_tokens < 0 || n_tokens > a.tokens - t_first)) {      // not rows of q
     if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
     return;
   }
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_rows_kernel(const __grid_c
   const auto token_of = [&](int c) { return (group * kCols + c) / R; };
   int keys = DECODE ? a.ctx[b] : (int)min((int64_t)first_pos + token_of(cols - 1) + 1, (int64_t)INT32_MAX);
   const int64_t room = (int64_t)a.width * a.cache.block;
-  if (keys > room || (!DECODE && (first_pos < 0 || n_tokens > a.max_len))) {
+  if (keys > room || (!DECODE && (first_pos < 0 || n_tokens > a.max_len || keys > a.max_ctx))) {
     if (tid == 0) report(a.status, NQB200_ERR_BAD_INDEX);
     keys = (int)min((int64_t)keys, room);
   }
@@ -807,6 +807,6 @@ extern "C" int nqb200_kv4_prompt_attention(const void* q, int64_t q_stride, cons
                             scratch, status, (cudaStream_t)stream);
   Args a = {};
   a.q = (const uint16_t*)q; a.stride = q_stride; a.cache = kv4::cache_of(cache); a.table = table; a.width = (int)table_width; a.cu = cu; a.pos0 = pos0;
-  a.out = (uint16_t*)out; a.heads = (int)num_q_heads; a.groups = (int)groups; a.tokens = (int)T; a.max_len = (int)max_len; a.scale = scale; a.status = status; a.shares = (float*)scratch;
+  a.out = (uint16_t*)out; a.heads = (int)num_q_heads; a.groups = (int)groups; a.tokens = (int)T; a.max_len = (int)max_len; a.max_ctx = (int)max_ctx; a.scale = scale; a.status = status; a.shares = (float*)scratch;
   return launch<false>(a, batch, T, max_ctx, dtype, (cudaStream_t)stream);
 }
