@@ -47,6 +47,7 @@ constexpr int kTileKeys = 128, kThreads = 640, kRows = 256;
 constexpr uint32_t kTileBytes = kTileKeys * kDim * 2, kBox = kTileKeys * 128;       // of K or V; of a block of 64 dimensions
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLag = 7.f, kRoom = 8.f;      // 2^(kLag + kRoom) is a number of float16
+constexpr float kLeast = 1e-37f;
 constexpr int kNone = 0x7FFFFFFF;
 
 struct alignas(16) TileInfo {
@@ -83,7 +84,7 @@ struct Params {
   TileInfo* info;        // [tile][kv head]
   float* shares;
   int heads, tokens, batch, parts, max_len, max_ctx, total;     // total: tiles that there is room for
-  float factor;          // scale log2 e, above 0 (a masked score stays minus infinity)
+  float factor;          // scale log2 e, above 0
   float sign;            // of the scale: the queries take it
   int* status;
 };
@@ -434,7 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
       ++exchanges;
       return got;
     };
-    const float row_factor = BF16 ? p.factor * s_row[q * 128 + row] : p.factor;
+    // (above 0 with all units in it, where a masked score stays minus infinity; the scores of queries and keys so small are nothing)
+    const float row_factor = BF16 ? fmaxf(p.factor * s_row[q * 128 + row], kLeast) : p.factor;
     float m = -INFINITY;
     uint64_t lsum = pair2(0.f, 0.f);
     // A row's reference goes from half to half in the order of their products: 0 and 1 of the first tile, 0 and 1 of the next, and so on,
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_co
         int wide = 0;
         if (SPECIAL) {
           const TileInfo t = p.info[(int64_t)(tile0 + j) * p.cache.kv_heads + blockIdx.y];
-          factor = fmaxf(factor * t.k, 1e-37f);
+          factor = fmaxf(factor * t.k, kLeast);
           wide = t.wide;
         }
         uint32_t r[2][32];     // the row's scores, all of this half
@@ -693,7 +695,7 @@ int prompt_umma(const uint16_t* q, int64_t q_stride, const nqb200_kv4* cache, co
   p.tiles = (uint8_t*)scratch; p.info = (TileInfo*)(p.tiles + tile_bytes(tiles, hk)); p.shares = (float*)((uint8_t*)p.info + info_bytes(tiles, hk));
   p.heads = (int)heads; p.tokens = (int)tokens; p.batch = (int)batch; p.max_len = (int)max_len; p.max_ctx = (int)max_ctx; p.total = (int)tiles;
   p.parts = parts_of(batch, max_len, max_ctx, heads, hk);
-  p.factor = fmaxf(fabsf(scale) * kLog2e, 1e-37f); p.sign = scale < 0.f ? -1.f : 1.f; p.status = status;
+  p.factor = fmaxf(fabsf(scale) * kLog2e, kLeast); p.sign = scale < 0.f ? -1.f : 1.f; p.status = status;
   const bool bf16 = dtype == NQB200_BF16;
   const dim3 expand((unsigned)((max_ctx + kTileKeys - 1) / kTileKeys), (unsigned)hk, (unsigned)batch);
   int rc = launch_overlapped(bf16 ? kv4_expand_kernel<true> : kv4_expand_kernel<false>, expand, dim3(512), 0, st, p);
