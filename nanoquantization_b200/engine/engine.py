@@ -151,6 +151,8 @@ class PagedKVCache:
 
 
 def _copy_rows(pools: list[torch.Tensor], pairs: list[tuple[int, int]]) -> None:
+    if not pools:
+        return
     sources, targets = [a for a, _ in pairs], [b for _, b in pairs]
     if pools[0].is_cuda:
         copy_pages(pools, sources, targets)
