@@ -230,6 +230,11 @@ def check_mixers(status: int) -> None:
         raise RuntimeError(f"nqb200_mixers: {_STATUS[status] if status < len(_STATUS) else 'unknown status'} (status {status})")
 
 
+def _status_word(device) -> torch.Tensor:
+    with torch.inference_mode(False):      # it is cleared in whatever mode the check comes
+        return torch.zeros(1, dtype=torch.int32, device=device)
+
+
 _mixer_status: dict[int, torch.Tensor] = {}
 
 
@@ -237,7 +242,7 @@ def mixer_status(dev: torch.device) -> torch.Tensor:
     """The device's status word for bounded waits of the mixer kernels (0: none gave up)."""
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     if idx not in _mixer_status:
-        _mixer_status[idx] = torch.zeros(1, dtype=torch.int32, device=dev)
+        _mixer_status[idx] = _status_word(dev)
     return _mixer_status[idx]
 
 
@@ -283,7 +288,7 @@ def cache_status(device: int) -> int | None:
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             return None
-        word = _cache_status[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+        word = _cache_status[device] = _status_word(f"cuda:{device}")
         torch.cuda.current_stream(device).synchronize()      # other streams' kernels may be the next to use it
     return word.data_ptr()
 
