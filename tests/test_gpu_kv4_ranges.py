@@ -162,3 +162,43 @@ def test_scores_far_from_zero(n, start, kv_heads, heads, shift, dtype):
     got = kv4.prompt_attention(q.flatten(1), heads, kc, vc, table, i32(0, n), i32(start), [n], [start])
     k, v = (ref.rows_of(c, rows, block, dtype) for c in (kc, vc))
     _each_close(got.view(n, heads, D), ref.attend(q.double(), k, v, start), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@torch.no_grad()
+def test_sequences_and_heads_of_different_sizes_in_one_call(dtype):
+    """Ordinary ones beside such of very large and very small values and keys, one with a value that is no number: each as by itself."""
+    from nanoquantization_b200 import _lib
+    from nanoquantization_b200.layers import kv4
+    lens, starts, kv_heads, heads, block = [300, 200, 260, 1], [40, 500, 0, 130], 2, 16, 64
+    far, near = (6e4, 1e-5) if dtype == torch.float16 else (1e30, 1e-12)
+    # of keys and values, by sequence and head
+    sizes = [((1.0, 1.0), (1.0, far)), ((1.0, 0.01), (near, 1.0)), ((1e-4, 1.0), (1.0, 0.0155)), ((1.0, 1.0), (far, near))]
+    assert _lib.load().nqb200_kv4_prompt_kernel_name(4, 761, 300, 700, 3 + 6 + 3 + 2, heads, kv_heads) == b"tiles_tcgen05"
+    g = torch.Generator(device=DEV).manual_seed(3)
+    need = [-(-(n + s) // block) for n, s in zip(lens, starts)]
+    order = torch.randperm(sum(need), generator=torch.Generator().manual_seed(3))
+    caches = [torch.full((sum(need), kv_heads, block * ref.TOKEN), 255, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    table, rows, at = torch.full((4, max(need)), -1, dtype=torch.int32), [], 0
+    for b, (n, s) in enumerate(zip(lens, starts)):
+        pages = order[at:at + need[b]]
+        at += need[b]
+        table[b, :need[b]] = pages.int()
+        rows.append((pages[torch.arange(n + s) // block] * block + torch.arange(n + s) % block).tolist())
+        for c, by in zip(caches, sizes[b]):
+            x = 2 * torch.rand(n + s, kv_heads, D, generator=g, device=DEV, dtype=torch.float64) - 1
+            ref.set_rows(c, rows[b], x * torch.tensor(by, device=DEV, dtype=torch.float64)[:, None], block, dtype)
+    bad = rows[1][600]
+    caches[1][..., block * 64:].unflatten(-1, (block, 8))[bad // block, 0, bad % block, 0:2] = 255            # the first group's scale, of small values
+    q = torch.randn(sum(lens), heads, D, generator=g, device=DEV).to(dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    cu = [0, 300, 500, 760, 761]
+    got = kv4.prompt_attention(q.flatten(1), heads, *caches, table.to(DEV), i32(cu), i32(starts), lens, starts).view(-1, heads, D)
+    for b, s in enumerate(starts):
+        k, v = (ref.rows_of(c, rows[b], block, dtype) for c in caches)
+        v = v.nan_to_num(0.0)
+        mine, want = got[cu[b]:cu[b + 1]].clone(), ref.attend(q[cu[b]:cu[b + 1]].double(), k, v, s)
+        if b == 1:
+            assert mine[100:, :8, :64].isnan().all() and int(mine.isnan().sum()) == 100 * 8 * 64
+            mine[100:, :8, :64] = want[100:, :8, :64].to(dtype)
+        _each_close(mine, want, dtype)
