@@ -23,10 +23,10 @@
 // Scores come out relative to a reference, which moves only when one is 8 (in log2 units) above it, found by one vote per 32 keys.  The warps meet in
 // shared memory, the CTAs of a cluster in distributed shared memory, several clusters of one sequence in a second launch; always in the same order.
 //
-// 64 sequences of 3500 keys on average, 64 heads over 8, bfloat16 (263 MB, 40 us at the copy rate): 74 us; float16 80; 45 of 1250, 32 heads over 8 (69
-// MB, 10.6 us) 26.5; one of 32000 17.7; one of 37 6.3.  The bytes come in at 3.6 TB/s at most: issue slots are 59 % busy (697 warp
-// instructions for 32 keys, of them 208 to take nibbles and parameters apart, 107 float arithmetic, 64 packed half, 32 products), the ALU
-// 51 %, the tensor pipe 21 %, DRAM 40 %, and CTAs of unequal sequences end at different times (IPC 2.3 while they run, 1.9 over all).
+// 64 sequences of 3500 keys on average, 64 heads over 8, bfloat16 (263 MB, 40 us at the copy rate): 73 us; float16 81; 45 of 1250, 32 heads over 8 (69
+// MB, 10.6 us) 26.4; one of 32000 17.8; one of 37 6.4.  The bytes come in at 3.6 TB/s at most: issue slots are 58 % busy (671 warp
+// instructions for 32 keys, of them about 200 to take nibbles and parameters apart, 107 float arithmetic, 64 packed half, 32 products), the ALU
+// 51 %, the tensor pipe 22 %, DRAM 40 %, and CTAs of unequal sequences end at different times (IPC 2.3 while they run, 1.9 over all).
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "kv4_attention.cuh"

@@ -24,10 +24,11 @@
 // rescaled, which hardly ever happens.  A half finds out by itself that its scores ask for no move, from their largest magnitude; that the
 // other half has not moved it learns from what that one hands on, in the order of the products.  The sum that a row is divided by takes the weights in float, before the product's rounding to 16 bits.
 //
-// One prompt of 8000 tokens, 32 heads over 8: 485 us (1.08 PFLOP/s of visible pairs, 0.66 of the measured peak; 560 back to back under the power
-// cap), of them about 10 for the first launch; 500 tokens behind 12000, 64 heads over 8, 211 (0.95 PFLOP/s: 128 CTAs on 148 SMs); 1000 tokens 33.
-// In between the tensor pipe is 53 % busy, the exponentials' pipe 55 %, issue slots 53 %: the chains meet at the pipes.  64 tokens take 16
-// us whatever they see: two launches, first bytes, one tile's chain.
+// One prompt of 8000 tokens, 32 heads over 8: 474 to 493 us, by the GPU (bfloat16; 1.10 PFLOP/s of visible pairs, 0.68 of the measured peak), 463 to
+// 473 in float16, 550 back to back under the power cap, of them about 10 for the first launch; 500 tokens behind 12000, 64 heads over 8, 208 (0.96
+// PFLOP/s: 128 CTAs on 148 SMs); 1000 tokens 35.  In between the tensor pipe is 54 % busy, the exponentials' pipe 56 %, issue slots 53 %: the chains
+// meet at the pipes.  64 tokens take 16 us by themselves (two launches, first bytes, one tile's chain) and 56 to 65 behind 16000, whose tiles
+// are written and read again.  4000 tokens 173; with all values in bfloat16 208, with all keys in units 186.
 //
 // Where the row tiles are fewer than the SMs, the keys are dealt to several CTAs, whose shares a third launch adds.
 //
