@@ -21,6 +21,7 @@ from .. import _lib
 DIM, TOKEN = 128, 72
 SPLIT_KEYS = 4096   # decode steps of tables for fewer keys need no scratch
 TILE = 128          # keys of a tile of prompt_attention, which take 512 bytes each per key/value head while it runs
+MOST_SEQUENCES, MOST_TILES = 65535, 1 << 24      # of a call of the library; more are taken in several goes
 MOST_SCRATCH = 1 << 30      # where they go into tiles, more sequences than fit are taken in several goes (one alone may take more)
 
 
@@ -151,15 +152,16 @@ def prompt_attention(q: torch.Tensor, num_q_heads: int, k_cache: torch.Tensor, v
     out = q.new_empty((T, num_q_heads * DIM))
     scale = DIM ** -0.5 if scale is None else scale
     with _lib.on_device(dev) as stream:
-        need = _lib.load().nqb200_kv4_prompt_scratch_bytes(B, T, max_len, max_ctx, tiles, num_q_heads, cache.kv_heads)
-        if need <= MOST_SCRATCH or B < 2:
+        fits = B < 2 or (B <= MOST_SEQUENCES and tiles <= MOST_TILES)
+        need = _lib.load().nqb200_kv4_prompt_scratch_bytes(B, T, max_len, max_ctx, tiles, num_q_heads, cache.kv_heads) if fits else 0
+        if fits and (need <= MOST_SCRATCH or B < 2):
             _prompt(q, out, num_q_heads, cache, k_cache, code, table, cu, pos0, B, max_len, max_ctx, tiles, scale, need, stream)
             return out
         room = max(1, MOST_SCRATCH // (TILE * 512 * cache.kv_heads))
         b = o = 0
         while b < B:
             e, t, n = b, 0, 0
-            while e < B and (t == 0 or t + (lens[e] + starts[e] + TILE - 1) // TILE <= room):
+            while e < B and e - b < MOST_SEQUENCES and (t == 0 or t + (lens[e] + starts[e] + TILE - 1) // TILE <= room):
                 t += (lens[e] + starts[e] + TILE - 1) // TILE if lens[e] else 0
                 n += lens[e]
                 e += 1
