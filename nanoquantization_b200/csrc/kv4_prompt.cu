@@ -5,8 +5,9 @@
 // and needs no tensor map.  float16 whatever the model's type: keys, values and weights in bfloat16 cost twice the error of the
 // result's own rounding (a prompt of 8000 tokens: 0.0031 in the 2-norm, 0.0017 so).  A bfloat16 model may have numbers that float16 would not
 // hold well.  A tile of keys is then in units of a power of two, and so is a query.  A tile of values has no unit, since weights times units would
-// lose what float16 does not hold of the product: it is in bfloat16 instead, and its weights are (values_fit).  So the precision of a row depends
-// on what it sees.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the
+// lose what float16 does not hold of the product: it is in bfloat16 instead, and its weights are (values_fit).  So values that a row does not see, or
+// gives no weight, cost it no precision.  Keys come from a norm, which keeps them within a few powers of ten of each other; in a tile whose largest is
+// beyond 2^15 those below 2^-28 of it are lost.  Rows behind a sequence's end are zeros, and so is a group of a value that is not finite: where the
 // first of those stands is noted, and the rows that see it get NaN at the end, and no other (a weight of 0 times NaN would be one).
 //
 // In the second a CTA takes 256 rows of a key/value head, as two tiles of 128: a row is a query head of a token, the heads of a group beside
